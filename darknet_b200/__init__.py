@@ -45,6 +45,27 @@ class ConvDesc(C.Structure):
                                        "batch_normalize", "activation", "xnor")]
 
 
+class RopeDesc(C.Structure):
+    """struct dnb_rope_desc."""
+    _fields_ = [("head_dim", C.c_int), ("heads", C.c_int), ("pairs", C.c_int * 3), ("frames", C.c_int), ("origin", C.c_int * 3),
+                ("interleaved", C.c_int), ("shared", C.c_int), ("base", C.c_float), ("scale", C.c_float * 3)]
+
+
+class AttentionDesc(C.Structure):
+    """struct dnb_attention_desc."""
+    _fields_ = [("heads", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int), ("scale", C.c_float)]
+
+
+class AttentionMask(C.Structure):
+    """struct dnb_attention_mask."""
+    _fields_ = [("lengths", C.c_void_p), ("mask", C.c_void_p), ("image_stride", C.c_longlong), ("query_stride", C.c_longlong)]
+
+
+class E4M3(C.Structure):
+    """struct dnb_e4m3."""
+    _fields_ = [("data", C.c_void_p), ("scales", C.c_void_p), ("pitch", C.c_int), ("group", C.c_int)]
+
+
 # name -> (restype, argtypes); every symbol include/darknet_b200.h declares
 _P, _I, _F = C.c_void_p, C.c_int, C.c_float
 _TP = C.POINTER(Tensor)
@@ -75,6 +96,16 @@ SIGNATURES = {
     "dnb_yolo_forward": (_I, [_TP, _TP, _I, _I, _P]),
     "dnb_avgpool_forward": (_I, [_TP, _TP, _P]),
     "dnb_softmax_forward": (_I, [_TP, _TP, _I, _F, _P]),
+    "dnb_rope_plan_create": (_I, [C.POINTER(RopeDesc), C.POINTER(_P)]),
+    "dnb_rope_plan_destroy": (None, [_P]),
+    "dnb_rope_forward": (_I, [_P, _TP, _P, _TP, _P]),
+    "dnb_attention_plan_create": (_I, [C.POINTER(AttentionDesc), C.POINTER(_P)]),
+    "dnb_attention_plan_destroy": (None, [_P]),
+    "dnb_attention_forward": (_I, [_P, _TP, _TP, _TP, C.POINTER(AttentionMask), _TP, _P]),
+    "dnb_attention_plan_check_status": (_I, [_P]),
+    "dnb_attention_plan_set_diagnostics": (_I, [_P, C.c_longlong, _I]),
+    "dnb_attention_plan_kernel": (C.c_char_p, [_P]),
+    "dnb_rmsnorm_forward": (_I, [_TP, _TP, _P, _F, _TP, _TP, C.POINTER(E4M3), _P]),
     "dnb_parse_network_cfg": (_I, [C.c_char_p, _I, _I, C.POINTER(_P)]),
     "dnb_parse_network_cfg_text": (_I, [C.c_char_p, _I, _I, C.POINTER(_P)]),
     "dnb_load_weights": (_I, [_P, C.c_char_p]),
@@ -131,8 +162,8 @@ def check(status: int) -> None:
         raise DarknetB200Error(status, lib().dnb_last_error().decode())
 
 
-from .api import (ConvPlan, Network, as_tensor, avgpool, convert, load_network, maxpool, network_predict,  # noqa: E402
-                  route, shortcut, softmax, upsample, yolo)
+from .api import (ConvPlan, CrossAttentionPlan, Network, RopePlan, as_tensor, avgpool, convert, load_network, maxpool,  # noqa: E402
+                  network_predict, rmsnorm, route, shortcut, softmax, upsample, yolo)
 
 __all__ = ["lib", "check", "Tensor", "ConvDesc", "ConvPlan", "Network", "load_network", "network_predict", "as_tensor",
-           "maxpool", "upsample", "shortcut", "route", "convert", "yolo", "avgpool", "softmax", "DarknetB200Error"]
+           "maxpool", "upsample", "shortcut", "route", "convert", "yolo", "avgpool", "softmax", "RopePlan", "CrossAttentionPlan", "rmsnorm", "DarknetB200Error"]

@@ -9,7 +9,7 @@ import ctypes as C
 
 import numpy as np
 
-from . import (ACTIVATIONS, BF16, F32, MODE_TF32, NCHW, NHWC, ConvDesc, Tensor, check, lib)
+from . import (ACTIVATIONS, BF16, E4M3, F32, MODE_TF32, NCHW, NHWC, AttentionDesc, AttentionMask, ConvDesc, RopeDesc, Tensor, check, lib)
 
 
 _current = None
@@ -139,6 +139,111 @@ def avgpool(x: Tensor, y: Tensor, stream=None):
 
 def softmax(x: Tensor, y: Tensor, groups: int = 1, temperature: float = 1.0, stream=None):
     check(lib().dnb_softmax_forward(C.byref(x), C.byref(y), groups, temperature, _stream(stream)))
+
+
+def _device_array(t, dtypes, shape, what):
+    """The address of a contiguous CUDA tensor of one of `dtypes` and of `shape`."""
+    if not t.is_cuda or t.dtype not in dtypes or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{what}: needs a contiguous CUDA tensor {list(shape)} of {' or '.join(str(d) for d in dtypes)}")
+    return t.data_ptr()
+
+
+def _ref(t):
+    return None if t is None else C.byref(t)
+
+
+class RopePlan:
+    """dnb_rope_plan: rotary positions with the axes (time, row, column)."""
+
+    def __init__(self, head_dim, heads, pairs, base=10000.0, interleaved=False, shared=True, frames=1, origin=(0, 0, 0), scale=(1.0, 1.0, 1.0)):
+        I3, F3 = C.c_int * 3, C.c_float * 3
+        self.desc = RopeDesc(head_dim, heads, I3(*pairs), frames, I3(*origin), int(interleaved), int(shared), base, F3(*scale))
+        self.handle = C.c_void_p()
+        check(lib().dnb_rope_plan_create(C.byref(self.desc), C.byref(self.handle)))
+
+    def forward(self, x: Tensor, y: Tensor, positions=None, stream=None):
+        """positions: int32 CUDA torch tensor [n * h * w, 3], or None for the tokens' places in the map."""
+        if positions is not None:
+            import torch
+            positions = _device_array(positions, (torch.int32,), (x.n * x.h * x.w, 3), "positions")
+        check(lib().dnb_rope_forward(self.handle, C.byref(x), positions, C.byref(y), _stream(stream)))
+
+    def close(self):
+        if self.handle:
+            lib().dnb_rope_plan_destroy(self.handle)
+            self.handle = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class CrossAttentionPlan:
+    """dnb_attention_plan: attention of query tokens to an encoder's states."""
+
+    def __init__(self, heads, kv_heads, head_dim, scale=0.0):
+        self.desc = AttentionDesc(heads, kv_heads, head_dim, scale)
+        self.handle = C.c_void_p()
+        check(lib().dnb_attention_plan_create(C.byref(self.desc), C.byref(self.handle)))
+
+    def forward(self, q: Tensor, k: Tensor, v: Tensor, y: Tensor, lengths=None, mask=None, stream=None):
+        """lengths: int32 CUDA torch tensor [n].  mask: bool or uint8 CUDA torch tensor [n, queries, keys], its keys contiguous; it may be
+        expanded along images and queries."""
+        masks = None
+        if lengths is not None or mask is not None:
+            import torch
+            masks = AttentionMask(None, None, 0, 0)
+            if lengths is not None:
+                masks.lengths = _device_array(lengths, (torch.int32,), (q.n,), "lengths")
+            if mask is not None:
+                keys = k.h * k.w
+                if not mask.is_cuda or mask.dtype not in (torch.bool, torch.uint8) or tuple(mask.shape) != (q.n, q.h * q.w, keys) or (keys > 1 and mask.stride(2) != 1):
+                    raise ValueError(f"mask: needs a CUDA tensor [{q.n}, {q.h * q.w}, {keys}] of bool or uint8 with contiguous keys")
+                masks.mask, masks.image_stride, masks.query_stride = mask.data_ptr(), mask.stride(0), mask.stride(1)
+            masks = C.byref(masks)
+        check(lib().dnb_attention_forward(self.handle, C.byref(q), C.byref(k), C.byref(v), masks, C.byref(y), _stream(stream)))
+
+    @property
+    def kernel(self) -> str:
+        """The kernel of the last forward."""
+        return lib().dnb_attention_plan_kernel(self.handle).decode()
+
+    def check_status(self):
+        check(lib().dnb_attention_plan_check_status(self.handle))
+
+    def set_diagnostics(self, wait_limit_cycles: int = 0, debug_bits: int = 0):
+        """As ConvPlan.set_diagnostics."""
+        check(lib().dnb_attention_plan_set_diagnostics(self.handle, wait_limit_cycles, debug_bits))
+
+    def close(self):
+        if self.handle:
+            lib().dnb_attention_plan_destroy(self.handle)
+            self.handle = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def rmsnorm(x: Tensor, y: Tensor | None = None, gain=None, eps=1e-6, residual: Tensor | None = None, total: Tensor | None = None,
+            e4m3=None, scales=None, group=0, stream=None):
+    """y = norm(x + residual) * gain; total: x + residual as stored; e4m3: the same as y in 8 bits.
+    gain: float32 CUDA torch tensor [c].  e4m3: float8_e4m3fn (or uint8) CUDA torch tensor [n, h, w, pitch] with scales, a float32 one
+    [n, h, w, groups]; group: channels that share a scale (32, 64, 128), or 0 for all."""
+    q = None
+    if gain is not None or e4m3 is not None:
+        import torch
+        if gain is not None:
+            gain = _device_array(gain, (torch.float32,), (x.c,), "gain")
+        if e4m3 is not None:
+            pitch = e4m3.shape[-1]
+            data = _device_array(e4m3, (torch.float8_e4m3fn, torch.uint8), (x.n, x.h, x.w, pitch), "e4m3")
+            q = C.byref(E4M3(data, _device_array(scales, (torch.float32,), (x.n, x.h, x.w, -(-x.c // group) if group > 0 else 1), "scales"), pitch, group))
+    check(lib().dnb_rmsnorm_forward(C.byref(x), _ref(residual), gain, eps, _ref(total), _ref(y), q, _stream(stream)))
 
 
 class Network:

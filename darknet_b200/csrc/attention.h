@@ -1,0 +1,35 @@
+// Internal argument blocks of the cross-attention kernels and the plan object.
+#pragma once
+#include "common.h"
+
+struct dnb_attention_plan {
+    dnb_attention_desc d;
+    int device;
+    int *status;            // device word: 0, or the code of the bounded wait that ran out
+    long long wait_limit;   // SM clock cycles
+    int debug;
+    const char *kernel;     // of the last forward, for logs and tests
+};
+
+namespace dnb {
+
+// One call.  Queries i of image n and head h: row n*lq + i of q, channels h*d ..; keys and values: row (kn == 1 ? 0 : n)*lk + j, channels h/group*d ..
+struct AttnArgs {
+    const void *q, *k, *v;
+    void *y;
+    int n, kn, lq, lk;
+    int heads, kv_heads, group, d;
+    int qp, kp, vp, yp;                     // pitches, elements
+    float scale;
+    const int32_t *lengths;                 // keys of each image, or null: all
+    const uint8_t *mask;                    // or null
+    long long mask_image, mask_query;       // its strides, bytes
+    int *status;
+    long long wait_limit;
+    int debug;
+};
+
+// ---- cross_attention.cu
+int launch_attention_simple(const AttnArgs &a, int dtype, cudaStream_t s);
+
+}  // namespace dnb

@@ -267,6 +267,92 @@ int dnb_avgpool_forward(const dnb_tensor *x, const dnb_tensor *y, void *stream);
 int dnb_softmax_forward(const dnb_tensor *x, const dnb_tensor *y, int groups, float temperature,
                         void *stream);
 
+/* ------------------------------------------------------------------ attention over feature maps */
+/* What a language or query head on a detector's feature map needs beside the 1x1 convolutions that project its
+ * tokens: rotary positions, attention to the map's pixels, and the norm between the blocks.  Channels-last tensors of
+ * one dtype (f32 or bf16); a token is a pixel, n * h * w of them, in the order of the memory.  Sums, softmax
+ * statistics and norms are fp32 whatever the dtype; an output is rounded once.  A tensor may be a channel range of a
+ * wider one (its own c, the wider one's cpitch): channels beyond its own, rounded up to eight, stay as they are.
+ * None of this has a counterpart in the reference. */
+
+#define DNB_ROPE_MAX_PAIRS 128
+
+/* Rotary positions.  The first `heads` heads of head_dim channels turn; the channels behind them pass.  Of each head
+ * P = pairs[0] + pairs[1] + pairs[2] pairs of channels turn, by the axes time, row and column in that order, and the
+ * other head_dim - 2P channels pass.  Pair i is the channels (i, i + P), or (2i, 2i + 1) where interleaved.
+ * It turns by position * scale[axis] * f, with f = base^(-i/P) (shared: one spectrum over all axes), or
+ * base^(-j/pairs[axis]) for the axis' own pair j.  A token's position is its place in the map (frame, row, column)
+ * plus origin, the frame counted within clips of `frames` consecutive images, or given with the call. */
+typedef struct dnb_rope_desc {
+    int head_dim, heads;
+    int pairs[3];
+    int frames;
+    int origin[3];
+    int interleaved, shared;
+    float base;
+    float scale[3];
+} dnb_rope_desc;
+
+typedef struct dnb_rope_plan dnb_rope_plan;
+
+/* Checks the geometry and works out the frequencies.  A plan holds no device memory: any device, any stream, any
+ * number of calls at once. */
+int dnb_rope_plan_create(const dnb_rope_desc *desc, dnb_rope_plan **plan);
+void dnb_rope_plan_destroy(dnb_rope_plan *plan);
+
+/* y = x with its heads turned; y may be x (then what passes is not touched).  positions: device int32
+ * [n * h * w][3], or NULL.  Angles are exact modulo a turn for every int32 position. */
+int dnb_rope_forward(const dnb_rope_plan *plan, const dnb_tensor *x, const int32_t *positions, const dnb_tensor *y,
+                     void *stream);
+
+/* Attention of q's tokens to k's and v's: heads query heads, kv_heads of keys and values, query head i reads head
+ * i / (heads / kv_heads).  scale 0 stands for 1 / sqrt(head_dim).  head_dim: a multiple of 8, at most 128. */
+typedef struct dnb_attention_desc {
+    int heads, kv_heads, head_dim;
+    float scale;
+} dnb_attention_desc;
+
+/* Which keys a query sees; device memory, either may be NULL.  lengths [n]: keys at and behind it are not there
+ * (below 0: none, above h * w: all).  mask: byte [image * image_stride + query * query_stride + key] of an image of q,
+ * non-zero where the query sees the key; a stride may be 0. */
+typedef struct dnb_attention_mask {
+    const int32_t *lengths;
+    const uint8_t *mask;
+    long long image_stride, query_stride;
+} dnb_attention_mask;
+
+typedef struct dnb_attention_plan dnb_attention_plan;
+
+int dnb_attention_plan_create(const dnb_attention_desc *desc, dnb_attention_plan **plan);
+void dnb_attention_plan_destroy(dnb_attention_plan *plan);
+
+/* y = softmax(scale q k^T) v.  q, y: [n][..][heads * head_dim]; k, v: [n or 1][..][kv_heads * head_dim], one image of
+ * states for all of q's where it is 1.  mask may be NULL.  A query that sees no key gets zeros.  y is no input's
+ * memory.  Keys and values at and behind an image's length are not used, whatever they hold, and nor are those that a
+ * mask with query_stride 0 hides; with a mask for each query, what only some of them may see has to be finite in v. */
+int dnb_attention_forward(dnb_attention_plan *plan, const dnb_tensor *q, const dnb_tensor *k, const dnb_tensor *v,
+                          const dnb_attention_mask *mask, const dnb_tensor *y, void *stream);
+
+/* dnb_conv_plan_check_status and dnb_conv_plan_set_diagnostics of an attention plan; the kernel of its last call. */
+int dnb_attention_plan_check_status(dnb_attention_plan *plan);
+int dnb_attention_plan_set_diagnostics(dnb_attention_plan *plan, long long wait_limit_cycles, int debug_bits);
+const char *dnb_attention_plan_kernel(const dnb_attention_plan *plan);
+
+/* An output in 8 bits: e4m3 values [n * h * w][pitch], 16-byte aligned, pitch >= c and a multiple of 8, and fp32
+ * scales [n * h * w][ceil(c / group)].  group: the channels that share a scale, 32, 64 or 128, or 0 for all of them. */
+typedef struct dnb_e4m3 {
+    void *data;
+    float *scales;
+    int pitch, group;
+} dnb_e4m3;
+
+/* s = x + residual;  y = s * rsqrt(mean over c of s^2 + eps) * gain;  q = y / scale with scale = max(max |y| of the
+ * group / 448, 2^-126).  residual, gain (device fp32 [c], or 1), sum (s as stored), y and q may each be NULL, but not
+ * all outputs, nor residual with a sum asked for.  The norm takes s before its rounding.  sum and y may each be x's or
+ * residual's own memory.  c: at most 32768 (bf16) or 16384 (f32). */
+int dnb_rmsnorm_forward(const dnb_tensor *x, const dnb_tensor *residual, const float *gain, float eps,
+                        const dnb_tensor *sum, const dnb_tensor *y, const dnb_e4m3 *q, void *stream);
+
 /* ------------------------------------------------------------------ network */
 typedef struct dnb_network dnb_network;
 
