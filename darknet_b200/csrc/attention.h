@@ -32,4 +32,8 @@ struct AttnArgs {
 // ---- cross_attention.cu
 int launch_attention_simple(const AttnArgs &a, int dtype, cudaStream_t s);
 
+// ---- cross_attention_tc.cu : bf16, on the tensor cores
+bool attention_tc_covers(const AttnArgs &a, int dtype);
+int launch_attention_tc(const AttnArgs &a, cudaStream_t s);
+
 }  // namespace dnb

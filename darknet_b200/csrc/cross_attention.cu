@@ -163,11 +163,15 @@ extern "C" int dnb_attention_forward(dnb_attention_plan *p, const dnb_tensor *q,
         if ((uintptr_t)mask->lengths % 4) DNB_FAIL(DNB_EINVAL, "attention: lengths must be 4-byte aligned");
         if (mask->mask && (mask->image_stride < 0 || mask->query_stride < 0)) DNB_FAIL(DNB_EINVAL, "attention: negative strides of the mask");
         a.lengths = mask->lengths;
-        a.mask = mask->mask; a.mask_image = mask->image_stride; a.mask_query = mask->query_stride;
+        a.mask = mask->mask; a.mask_image = mask->image_stride; a.mask_query = a.lq > 1 ? mask->query_stride : 0;   // one query: one mask for all of them
     }
     a.status = p->status; a.wait_limit = p->wait_limit; a.debug = p->debug;
     if (p->device < 0) DNB_FAIL(DNB_ECUDA, "attention: the plan was made without a CUDA device");
     DNB_TRY(check_current_device(p->device, "attention"));
+    if (attention_tc_covers(a, q->dtype)) {
+        p->kernel = "tc_bf16";
+        return launch_attention_tc(a, (cudaStream_t)stream);
+    }
     p->kernel = "simple";
     return launch_attention_simple(a, q->dtype, (cudaStream_t)stream);
 }

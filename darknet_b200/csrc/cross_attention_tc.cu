@@ -1,0 +1,560 @@
+// Cross attention of bf16 tensors on the 5th-generation tensor cores.
+//
+// A CTA holds two tiles of 128 query rows (a row: one query token of one head; the heads that share keys lie side by side, so that their keys
+// are loaded once) and walks over the keys in tiles of 128:
+//   S = Q K^T   tcgen05.mma, both operands in shared memory by TMA, S in TMEM (fp32)
+//   P = exp2(S * scale * log2 e - m)   a warpgroup a tile, a row a thread, out of TMEM and back into it as bf16
+//   O += P V    tcgen05.mma, P from TMEM, V from shared memory as it lies (channels innermost: a transposed operand), O in TMEM (fp32)
+// While one tile's warpgroup takes exponentials, the tensor cores multiply the other tile's: the two are never both idle.
+//
+// The running maximum m moves only when a row's largest score has outgrown it by more than 2^8 (every weight is then at most 256 times what
+// the largest should be, far inside bf16's and fp32's range); until then O needs no correction.  The sum of the weights is kept in fp32 of the
+// unrounded weights; a weight is rounded to bf16 (half a step: 2^-8 of itself) as the operand of the second product, and nothing else is rounded
+// before the output.
+//
+// Few rows: the keys of one pair of tiles are split over the CTAs of a cluster, which join their sums through distributed shared memory: no
+// workspace, one launch, the same order of additions every time.
+#include <atomic>
+
+#include "attention.h"
+#include "device_utils.cuh"
+#include "tc_ptx.cuh"
+
+namespace dnb {
+
+int encode_tensor_map(CUtensorMap *map, int elem_kind, int rank, void *base, const uint64_t *dims, const uint64_t *strides_bytes, const uint32_t *box, int swizzle_bytes);
+size_t tmem_smem(size_t bytes, int cols);
+int conv_tc_max_smem();
+
+namespace {
+
+constexpr int THREADS = 320;                      // two warpgroups of softmax, a warp for the loads, one for the products
+constexpr int MAX_STAGES = 12;
+constexpr uint32_t BOX_BYTES = 128 * 128;         // 64 channels of 128 rows
+constexpr float MOVE = 8.f;                       // how far (log2) scores may outgrow the running maximum
+
+enum { AT_QUERIES = 201, AT_SLOT, AT_KEYS, AT_VALUES, AT_SCORES, AT_WEIGHTS, AT_OUTPUT, AT_SMEM_BASE };
+
+struct Shared {
+    uint64_t q_full, full[MAX_STAGES], empty[MAX_STAGES], s_full[2], p_full[2], o_full[2];
+    uint32_t tmem_base;
+    int abort_flag;
+    float top[256], sum[256];                     // of the rows, for the join
+};
+
+struct alignas(64) TcAttnArgs {
+    CUtensorMap tmq, tmk, tmv;
+    AttnArgs a;
+    int q_tokens;          // query tokens of a tile
+    int q_tiles;           // pairs of tiles an image and key head
+    int splits;            // CTAs of a cluster
+    float scale_log2;      // |scale| * log2 e
+    int negate;            // scale < 0: the products with -Q
+};
+
+__device__ __forceinline__ uint64_t pack2(float lo, float hi)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi)
+{
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// 32 columns of this warp's 32 lanes
+__device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t *r)
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+          "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
+          "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(at));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t *r)
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+          "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// V as it lies in shared memory: rows of 64 channels (128 bytes, swizzled), a key each: N is contiguous.  Blocks of 64 channels are a box
+// apart, groups of eight keys 1024 bytes.
+__device__ __forceinline__ uint64_t desc_values(uint32_t addr)
+{
+    uint64_t d = (uint64_t)((addr & 0x3FFFF) >> 4);
+    d |= (uint64_t)(BOX_BYTES >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+__device__ __forceinline__ void umma_from_tmem(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ float4 ld_peer(uint32_t addr, uint32_t rank)
+{
+    float4 v;
+    asm volatile(
+        "{\n\t.reg .b32 at;\n\t"
+        "mapa.shared::cluster.u32 at, %4, %5;\n\t"
+        "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [at];\n\t}"
+        : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr), "r"(rank) : "memory");
+    return v;
+}
+__device__ __forceinline__ float ld_peer1(uint32_t addr, uint32_t rank)
+{
+    float v;
+    asm volatile("{\n\t.reg .b32 at;\n\tmapa.shared::cluster.u32 at, %1, %2;\n\tld.shared::cluster.f32 %0, [at];\n\t}" : "=f"(v) : "r"(addr), "r"(rank) : "memory");
+    return v;
+}
+
+// DP: channels of a head as they lie in shared memory, 64 or 128 (TMA fills what the head does not have with zeros).
+template <int DP> struct Cfg {
+    static constexpr int BOXES = DP / 64;
+    static constexpr uint32_t TILE_BYTES = BOXES * BOX_BYTES;
+    static constexpr int STAGES = DP == 128 ? 5 : 12;
+    static constexpr uint32_t WORK = 2 * TILE_BYTES + STAGES * TILE_BYTES;
+    static constexpr int PITCH = DP + 4;          // of a row of sums, for the join
+    static_assert(256 * PITCH * 4 <= WORK && STAGES <= MAX_STAGES, "the rows' sums fit where the operands were");
+    static_assert(WORK + sizeof(Shared) <= 232448, "");
+};
+
+template <int DP, bool MASK>
+__global__ void __launch_bounds__(THREADS, 1)
+attention_tc_kernel(const __grid_constant__ TcAttnArgs t)
+{
+    using C = Cfg<DP>;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    const AttnArgs &a = t.a;
+    const uint32_t smem = smem_u32(smem_raw);
+    if (smem & 1023u) {
+        if (threadIdx.x == 0) atomicCAS(a.status, 0, AT_SMEM_BASE);
+        return;
+    }
+    Shared *sh = reinterpret_cast<Shared *>(smem_raw + C::WORK);
+    volatile int *abort_flag = &sh->abort_flag;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    const uint32_t q_smem = smem, ring = smem + 2 * C::TILE_BYTES;
+
+    const int rank = (int)(blockIdx.x % (unsigned)t.splits), job = (int)(blockIdx.x / (unsigned)t.splits);
+    const int q_tile = job % t.q_tiles, kv_head = job / t.q_tiles % a.kv_heads, image = job / t.q_tiles / a.kv_heads;
+    const int token0 = q_tile * 2 * t.q_tokens;
+    const int sides = token0 + t.q_tokens < a.lq ? 2 : 1;
+
+    if (tid == 0) {
+        mbar_init(smem_u32(&sh->q_full), 1);
+        for (int i = 0; i < C::STAGES; ++i) {
+            mbar_init(smem_u32(&sh->full[i]), 1);
+            mbar_init(smem_u32(&sh->empty[i]), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&sh->s_full[i]), 1);
+            mbar_init(smem_u32(&sh->p_full[i]), 4);
+            mbar_init(smem_u32(&sh->o_full[i]), 1);
+        }
+        sh->abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh->tmem_base)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    grid_dependency_wait();
+    launch_dependents_if_small();
+    const uint32_t tmem = sh->tmem_base;
+    auto s_cols = [&](int s) { return tmem + 128 * s; };
+    auto o_cols = [&](int s) { return tmem + 256 + DP * s; };
+
+    int keys = a.lk;
+    if (a.lengths) keys = min(max(a.lengths[image], 0), a.lk);
+    const int all = (keys + 127) >> 7, per = (all + t.splits - 1) / t.splits;
+    const int t0 = min(rank * per, all), tiles = min(t0 + per, all) - t0;
+
+    if (warp == 8) {
+        // ---------------------------------------------------------------- loads
+        if (tiles > 0) {
+            const int kv_image = a.kn == 1 ? 0 : image;
+            const uint32_t q_bytes = (uint32_t)(a.group * t.q_tokens) * 128u;
+            const uint32_t qbar = smem_u32(&sh->q_full);
+            if (elect_one()) {
+                mbar_expect_tx(qbar, q_bytes * C::BOXES * sides);
+                for (int s = 0; s < sides; ++s)
+                    for (int b = 0; b < C::BOXES; ++b)
+                        tma_load_4d(q_smem + s * C::TILE_BYTES + b * BOX_BYTES, &t.tmq, qbar, b * 64, kv_head * a.group, token0 + s * t.q_tokens, image);
+            }
+            int stage = 0;
+            uint32_t phase = 0;
+            for (int i = 0; i < 2 * tiles; ++i) {
+                const uint32_t full = smem_u32(&sh->full[stage]);
+                if (!mbar_wait_warp(smem_u32(&sh->empty[stage]), phase ^ 1, abort_flag, a.status, AT_SLOT, a.wait_limit)) break;
+                if (elect_one() && !(a.debug & 32 && i == 1)) {
+                    mbar_expect_tx(full, C::TILE_BYTES);
+                    for (int b = 0; b < C::BOXES; ++b)
+                        tma_load_4d(ring + stage * C::TILE_BYTES + b * BOX_BYTES, i & 1 ? &t.tmv : &t.tmk, full, b * 64, kv_head, (t0 + i / 2) * 128, kv_image);
+                }
+                if (++stage == C::STAGES) { stage = 0; phase ^= 1; }
+            }
+        }
+    } else if (warp == 9) {
+        // ---------------------------------------------------------------- products
+        bool ok = tiles > 0 && mbar_wait_warp(smem_u32(&sh->q_full), 0, abort_flag, a.status, AT_QUERIES, a.wait_limit);
+        const int qk_steps = (a.d + 15) >> 4;
+        const uint32_t idesc_qk = mma_idesc<MMA_BF16>(128, 128) | (t.negate ? 1u << 13 : 0u);                     // bit 13: A, negated
+        const uint32_t idesc_pv = mma_idesc<MMA_BF16>(128, (uint32_t)(qk_steps * 16)) | 1u << 16;                 // bit 16: B's rows are contiguous along N
+        auto scores = [&](int s, uint32_t k_smem) {
+            if (elect_one()) {
+                for (int i = 0; i < qk_steps; ++i) {
+                    const uint32_t off = (i >> 2) * BOX_BYTES + (i & 3) * 32;
+                    umma<MMA_BF16>(s_cols(s), make_smem_desc(q_smem + s * C::TILE_BYTES + off, 128), make_smem_desc(k_smem + off, 128), idesc_qk, i > 0);
+                }
+                umma_commit(smem_u32(&sh->s_full[s]));
+            }
+        };
+        // slot 2j of the ring is K's tile j, slot 2j + 1 V's
+        int stage = 0;
+        uint32_t phase = 0;
+        auto next = [&]() { if (++stage == C::STAGES) { stage = 0; phase ^= 1; } };
+        if (ok) ok = mbar_wait_warp(smem_u32(&sh->full[0]), 0, abort_flag, a.status, AT_KEYS, a.wait_limit);
+        if (ok) {
+            for (int s = 0; s < sides; ++s) scores(s, ring);
+            if (elect_one()) umma_commit(smem_u32(&sh->empty[0]));
+            next();
+        }
+        for (int j = 0; ok && j < tiles; ++j) {
+            const int v_stage = stage;
+            const uint32_t v_phase = phase;
+            next();
+            const int k_stage = stage;
+            const uint32_t k_phase = phase;
+            const bool more = j + 1 < tiles;
+            if (more) next();
+            if (!mbar_wait_warp(smem_u32(&sh->full[v_stage]), v_phase, abort_flag, a.status, AT_VALUES, a.wait_limit)) { ok = false; break; }
+            for (int s = 0; s < sides; ++s) {
+                if (!mbar_wait_warp(smem_u32(&sh->p_full[s]), j & 1, abort_flag, a.status, AT_WEIGHTS, a.wait_limit)) { ok = false; break; }
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t v_smem = ring + v_stage * C::TILE_BYTES;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) umma_from_tmem(o_cols(s), s_cols(s) + 8 * i, desc_values(v_smem + i * 2048), idesc_pv, j > 0 || i > 0);
+                    if (s == sides - 1) umma_commit(smem_u32(&sh->empty[v_stage]));
+                    if (!more) umma_commit(smem_u32(&sh->o_full[s]));
+                }
+                if (more) {
+                    if (s == 0 && !mbar_wait_warp(smem_u32(&sh->full[k_stage]), k_phase, abort_flag, a.status, AT_KEYS, a.wait_limit)) { ok = false; break; }
+                    scores(s, ring + k_stage * C::TILE_BYTES);
+                    if (s == sides - 1 && elect_one()) umma_commit(smem_u32(&sh->empty[k_stage]));
+                }
+            }
+        }
+    }
+
+    __syncwarp();
+
+    // ---------------------------------------------------------------- softmax: a row a thread
+    const int s = warp >> 2, row = tid & 127;
+    const bool mine = warp < 4 * sides && warp < 8;
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;                  // this warp's lanes of TMEM
+    const int r_token = token0 + s * t.q_tokens + row / a.group;
+    const bool valid = mine && row < t.q_tokens * a.group && r_token < a.lq;
+    float top = -INFINITY, sum = 0.f;
+    bool ok = true;
+    if (mine) {
+        const float scale = t.scale_log2;
+        const uint8_t *mask = nullptr;
+        if (MASK) mask = a.mask + (long long)image * a.mask_image + (valid ? r_token : a.lq - 1) * a.mask_query;
+        int stage = 1;
+        uint32_t phase = 0;                                             // of V's slots
+        for (int j = 0; j < tiles; ++j) {
+            const int key0 = (t0 + j) * 128, left = keys - key0;
+            uint32_t bits[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+            if (MASK) {
+                // The rows' masks, one row after another, 32 keys a load; rows of one query (heads that share keys) share the load.
+                const uint8_t *last = nullptr;
+                uint32_t now[4] = {0, 0, 0, 0};
+                for (int i = 0; i < 32; ++i) {
+                    const uint8_t *p = reinterpret_cast<const uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mask), i));
+                    if (p != last) {
+                        last = p;
+                        p += key0;
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            const int c = lane + 32 * w;
+                            now[w] = __ballot_sync(0xffffffffu, c < left && p[c] != 0);
+                        }
+                    }
+                    if (lane == i) { bits[0] = now[0]; bits[1] = now[1]; bits[2] = now[2]; bits[3] = now[3]; }
+                }
+            } else if (left < 128) {
+#pragma unroll
+                for (int w = 0; w < 4; ++w) bits[w] = left >= 32 * w + 32 ? 0xffffffffu : left > 32 * w ? (1u << (left - 32 * w)) - 1u : 0u;
+            }
+            if (!mbar_wait(smem_u32(&sh->s_full[s]), j & 1, abort_flag, a.status, AT_SCORES, 0, a.wait_limit)) { ok = false; break; }
+            tc_fence_after();
+            uint32_t v[128];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_ld32(s_cols(s) + lanes + 32 * c, v + 32 * c);
+            tmem_ld_wait();
+            if (MASK || left < 128) {
+#pragma unroll
+                for (int c = 0; c < 128; ++c)
+                    if (!(bits[c >> 5] >> (c & 31) & 1)) v[c] = 0xff800000u;
+            }
+            float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int c = 0; c < 128; ++c) most[c & 3] = fmaxf(most[c & 3], __uint_as_float(v[c]));
+            const float grown = fmaxf(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])), top);
+            if (__any_sync(0xffffffffu, (grown - top) * scale > MOVE)) {
+                const float shrink = grown == top ? 1.f : ex2((top - grown) * scale);
+                if (j > 0) {
+                    // every product of the tile before has retired: the scores' barrier came after them
+#pragma unroll 1
+                    for (int c = 0; c < DP; c += 16) {
+                        uint32_t o[16];
+                        tmem_ld16(o_cols(s) + lanes + c, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink);
+                        tmem_st16(o_cols(s) + lanes + c, o);
+                    }
+                }
+                sum *= shrink;
+                top = grown;
+            }
+            const float base = top == -INFINITY ? 0.f : top * scale;
+            const uint64_t scale2 = pack2(scale, scale), base2 = pack2(-base, -base);
+            uint64_t sums[2] = {0, 0};
+#pragma unroll
+            for (int c = 0; c < 128; c += 32) {
+                uint32_t p[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    float x, y;
+                    unpack2(fma2(pack2(__uint_as_float(v[c + 2 * e]), __uint_as_float(v[c + 2 * e + 1])), scale2, base2), x, y);
+                    x = ex2(x);
+                    y = ex2(y);
+                    sums[e & 1] = add2(sums[e & 1], pack2(x, y));
+                    p[e] = pack_bf16(x, y);
+                }
+                tmem_st16(s_cols(s) + lanes + c / 2, p);
+            }
+            float x0, x1, x2, x3;
+            unpack2(sums[0], x0, x1);
+            unpack2(sums[1], x2, x3);
+            sum += (x0 + x1) + (x2 + x3);
+            // Values that no weight reaches may be anything, and zero times infinity is no number: zeros in their place.  (Both tiles write them.)
+            if ((left < 128 && keys < a.lk) || (MASK && a.mask_query == 0)) {
+                if (!mbar_wait(smem_u32(&sh->full[stage]), phase, abort_flag, a.status, AT_VALUES, 0, a.wait_limit)) { ok = false; break; }
+                bool hidden = row >= left;
+                if (MASK && a.mask_query == 0 && !hidden) hidden = mask[key0 + row] == 0;
+                if (hidden) {
+                    const uint32_t at = 2 * C::TILE_BYTES + stage * C::TILE_BYTES + row * 128;
+#pragma unroll
+                    for (int b = 0; b < C::BOXES; ++b)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) *reinterpret_cast<uint4 *>(smem_raw + at + b * BOX_BYTES + e * 16) = make_uint4(0, 0, 0, 0);
+                }
+                fence_async_smem();
+            }
+            stage += 2;
+            if (stage >= C::STAGES) { stage -= C::STAGES; phase ^= 1; }
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sh->p_full[s]));
+        }
+        if (ok && tiles > 0) {
+            ok = mbar_wait(smem_u32(&sh->o_full[s]), 0, abort_flag, a.status, AT_OUTPUT, 0, a.wait_limit);
+            tc_fence_after();
+        }
+    }
+
+    const bool wide = a.d % 16 == 0 && a.yp % 16 == 0 && (uintptr_t)a.y % 32 == 0;   // whole 32-byte sectors
+    __nv_bfloat16 *y = (__nv_bfloat16 *)a.y + ((size_t)image * a.lq + r_token) * a.yp + (kv_head * a.group + row % a.group) * a.d;
+    if (t.splits == 1) {
+        if (mine && ok) {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll 1
+            for (int c = 0; c < a.d; c += 16) {
+                uint32_t o[16], p[8];
+                if (tiles > 0) {
+                    tmem_ld16(o_cols(s) + lanes + c, o);
+                    tmem_ld_wait();
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    p[e] = tiles > 0 && sum != 0.f ? pack_bf16(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv) : 0u;
+                if (valid) {
+                    if (wide) st_global_32(y + c, p);
+                    else {
+                        *reinterpret_cast<uint4 *>(y + c) = make_uint4(p[0], p[1], p[2], p[3]);
+                        if (c + 8 < a.d) *reinterpret_cast<uint4 *>(y + c + 8) = make_uint4(p[4], p[5], p[6], p[7]);
+                    }
+                }
+            }
+        }
+        __syncthreads();
+    } else {
+        __syncthreads();                                                // the other tile's products have read their operands too
+        float *rows = reinterpret_cast<float *>(smem_raw);
+        if (mine) {
+            sh->top[s * 128 + row] = top;
+            sh->sum[s * 128 + row] = sum;
+            if (tiles > 0 && ok) {
+#pragma unroll 1
+                for (int c = 0; c < DP; c += 16) {
+                    uint32_t o[16];
+                    tmem_ld16(o_cols(s) + lanes + c, o);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4)
+                        *reinterpret_cast<uint4 *>(rows + (s * 128 + row) * C::PITCH + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                }
+            }
+        }
+        cluster_sync_all();
+        // Rows rank, rank + splits, ... of the pair of tiles, `splits` threads a row: the shares' sums, in the order of the keys.
+        if (tid < 128 * sides && !*abort_flag) {
+            const int part = tid % t.splits, r = tid / t.splits * t.splits + rank, side = r >> 7, in_tile = r & 127;
+            const int token = token0 + side * t.q_tokens + in_tile / a.group;
+            if (in_tile < t.q_tokens * a.group && token < a.lq) {
+                float most = -INFINITY, weight[8], total = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (i < t.splits) most = fmaxf(most, ld_peer1(smem_u32(&sh->top[r]), i));
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (i < t.splits) {
+                        const float m = ld_peer1(smem_u32(&sh->top[r]), i), l = ld_peer1(smem_u32(&sh->sum[r]), i);
+                        weight[i] = l == 0.f ? 0.f : m == most ? 1.f : ex2((m - most) * t.scale_log2);   // no weights: its rows hold nothing
+                        total += l * weight[i];
+                    }
+                const float inv = total == 0.f ? 0.f : 1.f / total;
+                __nv_bfloat16 *out = (__nv_bfloat16 *)a.y + ((size_t)image * a.lq + token) * a.yp + (kv_head * a.group + in_tile % a.group) * a.d;
+                for (int c = part * 8; c < a.d; c += t.splits * 8) {
+                    float o[8] = {};
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (i < t.splits && weight[i] != 0.f) {
+                            const float4 x = ld_peer(smem_u32(rows + r * C::PITCH + c), i), z = ld_peer(smem_u32(rows + r * C::PITCH + c + 4), i);
+                            o[0] = fmaf(x.x, weight[i], o[0]); o[1] = fmaf(x.y, weight[i], o[1]); o[2] = fmaf(x.z, weight[i], o[2]); o[3] = fmaf(x.w, weight[i], o[3]);
+                            o[4] = fmaf(z.x, weight[i], o[4]); o[5] = fmaf(z.y, weight[i], o[5]); o[6] = fmaf(z.z, weight[i], o[6]); o[7] = fmaf(z.w, weight[i], o[7]);
+                        }
+                    *reinterpret_cast<uint4 *>(out + c) = make_uint4(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv),
+                                                                     pack_bf16(o[4] * inv, o[5] * inv), pack_bf16(o[6] * inv, o[7] * inv));
+                }
+            }
+        }
+        cluster_sync_all();                                             // a peer's rows are read until here
+    }
+    if (*abort_flag) {                                                  // loads and products in flight end before their memory goes
+        const long long begin = clock64();
+        while (clock64() - begin < 4000000LL) { }
+    }
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+typedef void (*Kernel)(TcAttnArgs);
+
+int prepare(Kernel kern, int which)
+{
+    static std::atomic<bool> done[64][4];
+    int dev = 0;
+    DNB_CUDA(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64) DNB_FAIL(DNB_ECUDA, "attention: device %d", dev);
+    if (done[dev][which].load(std::memory_order_acquire)) return DNB_OK;
+    DNB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, conv_tc_max_smem()));
+    done[dev][which].store(true, std::memory_order_release);
+    return DNB_OK;
+}
+
+}  // namespace
+
+bool attention_tc_covers(const AttnArgs &a, int dtype)
+{
+    const long long jobs = (long long)a.n * a.kv_heads * ((a.lq + 127) / 128) * 128;
+    return dtype == DNB_BF16 && a.d <= 128 && a.group <= 128 && jobs < 1LL << 28;
+}
+
+int launch_attention_tc(const AttnArgs &a, cudaStream_t stream)
+{
+    TcAttnArgs t;
+    t.a = a;
+    if (!t.a.wait_limit) t.a.wait_limit = WAIT_LIMIT_CYCLES;
+    t.q_tokens = 128 / a.group;
+    t.q_tiles = (a.lq + 2 * t.q_tokens - 1) / (2 * t.q_tokens);
+    t.scale_log2 = (a.scale < 0.f ? -a.scale : a.scale) * 1.4426950408889634f;
+    t.negate = a.scale < 0.f;
+    auto map = [&](CUtensorMap *m, const void *data, int heads, int pitch, int tokens, int images, int box_heads, int box_tokens) {
+        const uint64_t dims[4] = {(uint64_t)a.d, (uint64_t)heads, (uint64_t)tokens, (uint64_t)images};
+        const uint64_t strides[3] = {(uint64_t)a.d * 2, (uint64_t)pitch * 2, (uint64_t)tokens * pitch * 2};
+        const uint32_t box[4] = {64, (uint32_t)box_heads, (uint32_t)box_tokens, 1};
+        return encode_tensor_map(m, 1, 4, const_cast<void *>(data), dims, strides, box, 128);
+    };
+    DNB_TRY(map(&t.tmq, a.q, a.heads, a.qp, a.lq, a.n, a.group, t.q_tokens));
+    DNB_TRY(map(&t.tmk, a.k, a.kv_heads, a.kp, a.lk, a.kn, 1, 128));
+    DNB_TRY(map(&t.tmv, a.v, a.kv_heads, a.vp, a.lk, a.kn, 1, 128));
+    // Fewer CTAs than SMs: split the keys, two tiles of them a CTA at least.
+    const long long jobs = (long long)a.n * a.kv_heads * t.q_tiles;
+    const int key_tiles = (a.lk + 127) / 128;
+    t.splits = 1;
+    while (t.splits < 8 && jobs * t.splits * 2 <= sm_count() && key_tiles >= t.splits * 4) t.splits *= 2;
+    const int which = (a.d > 64 ? 2 : 0) + (a.mask ? 1 : 0);
+    const Kernel kern = which == 0 ? attention_tc_kernel<64, false> : which == 1 ? attention_tc_kernel<64, true> : which == 2 ? attention_tc_kernel<128, false> : attention_tc_kernel<128, true>;
+    DNB_TRY(prepare(kern, which));
+    cudaLaunchAttribute attrs[2];
+    attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[0].val.programmaticStreamSerializationAllowed = pdl_enabled() && jobs * t.splits <= EARLY_BLOCKS ? 1 : 0;
+    attrs[1].id = cudaLaunchAttributeClusterDimension;
+    attrs[1].val.clusterDim.x = (unsigned)t.splits; attrs[1].val.clusterDim.y = 1; attrs[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(jobs * t.splits));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = tmem_smem((a.d > 64 ? Cfg<128>::WORK : Cfg<64>::WORK) + sizeof(Shared), 512);
+    cfg.stream = stream;
+    cfg.attrs = attrs;
+    cfg.numAttrs = 2;
+    DNB_CUDA(cudaLaunchKernelEx(&cfg, kern, t));
+    DNB_LAUNCH_CHECK("attention");
+    return DNB_OK;
+}
+
+}  // namespace dnb
