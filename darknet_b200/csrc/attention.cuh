@@ -1,0 +1,92 @@
+// Device code that the cross-attention kernels share.
+#pragma once
+#include "attention.h"
+#include "device_utils.cuh"
+#include "tc_ptx.cuh"
+
+namespace dnb {
+
+// What a wait that ran out was for.
+enum { AT_QUERIES = 201, AT_SLOT, AT_KEYS, AT_VALUES, AT_SCORES, AT_WEIGHTS, AT_OUTPUT, AT_SMEM_BASE };
+
+// 2^x, as the hardware's one instruction has it (2 ulp); 0 below 2^-126.
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi)
+{
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+__device__ __forceinline__ float4 ld_peer(uint32_t addr, uint32_t rank)
+{
+    float4 v;
+    asm volatile(
+        "{\n\t.reg .b32 at;\n\t"
+        "mapa.shared::cluster.u32 at, %4, %5;\n\t"
+        "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [at];\n\t}"
+        : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr), "r"(rank) : "memory");
+    return v;
+}
+__device__ __forceinline__ float ld_peer1(uint32_t addr, uint32_t rank)
+{
+    float v;
+    asm volatile("{\n\t.reg .b32 at;\n\tmapa.shared::cluster.u32 at, %1, %2;\n\tld.shared::cluster.f32 %0, [at];\n\t}" : "=f"(v) : "r"(addr), "r"(rank) : "memory");
+    return v;
+}
+
+// The keys that CTA `rank` of `splits` walks over, in tiles of `size`: [first, first + count) of an image's `keys`.
+__device__ __forceinline__ void share_of_keys(int keys, int size, int rank, int splits, int &first, int &count)
+{
+    const int all = (keys + size - 1) / size, per = (all + splits - 1) / splits;
+    first = min(rank * per, all);
+    count = min(first + per, all) - first;
+}
+
+// Joins the rows that the CTAs of a cluster hold of the same queries: in every CTA, at the same addresses of shared memory, row r's sum of weighted
+// values at rows + r * pitch floats, its largest scaled score (log2) in tops[r] and its sum of weights in sums[r] (0: its row holds nothing).
+// Eight channels an item, the items dealt out over the cluster's threads; the additions in the order of the ranks, which is the keys'.
+// out(r): where row r's d channels go, or null.
+template <typename T, typename Out>
+__device__ __forceinline__ void join_rows(uint32_t rows, int pitch, uint32_t tops, uint32_t sums, int count, int d, int rank, int splits, int tid, int threads, Out out)
+{
+    const int chunks = d / 8;
+    for (int i = tid * splits + rank; i < count * chunks; i += threads * splits) {
+        const int r = i / chunks, c = (i - r * chunks) * 8;
+        T *to = out(r);
+        if (!to) continue;
+        float most = -INFINITY, top[8], weight[8], total = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k < splits) {
+                top[k] = ld_peer1(tops + 4 * r, k);
+                weight[k] = ld_peer1(sums + 4 * r, k);
+                most = fmaxf(most, top[k]);
+            }
+        float o[8] = {};
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k < splits && weight[k] != 0.f) {
+                const float w = top[k] == most ? 1.f : ex2(top[k] - most);
+                total += weight[k] * w;
+                const float4 x = ld_peer(rows + (r * pitch + c) * 4, k), z = ld_peer(rows + (r * pitch + c + 4) * 4, k);
+                o[0] = fmaf(x.x, w, o[0]); o[1] = fmaf(x.y, w, o[1]); o[2] = fmaf(x.z, w, o[2]); o[3] = fmaf(x.w, w, o[3]);
+                o[4] = fmaf(z.x, w, o[4]); o[5] = fmaf(z.y, w, o[5]); o[6] = fmaf(z.z, w, o[6]); o[7] = fmaf(z.w, w, o[7]);
+            }
+        const float inv = total == 0.f ? 0.f : 1.f / total;
+        if constexpr (sizeof(T) == 2) {
+            *reinterpret_cast<uint4 *>(to + c) = make_uint4(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv), pack_bf16(o[4] * inv, o[5] * inv),
+                                                            pack_bf16(o[6] * inv, o[7] * inv));
+        } else {
+            *reinterpret_cast<float4 *>(to + c) = make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+            *reinterpret_cast<float4 *>(to + c + 4) = make_float4(o[4] * inv, o[5] * inv, o[6] * inv, o[7] * inv);
+        }
+    }
+}
+
+}  // namespace dnb

@@ -36,4 +36,12 @@ int launch_attention_simple(const AttnArgs &a, int dtype, cudaStream_t s);
 bool attention_tc_covers(const AttnArgs &a, int dtype);
 int launch_attention_tc(const AttnArgs &a, cudaStream_t s);
 
+// ---- cross_attention_rows.cu : bf16, up to 16 rows a key head
+bool attention_rows_covers(const AttnArgs &a, int dtype);
+int launch_attention_rows(const AttnArgs &a, cudaStream_t s);
+
+// ---- cross_attention_f32.cu : f32, on the CUDA cores
+bool attention_f32_covers(const AttnArgs &a, int dtype);
+int launch_attention_f32(const AttnArgs &a, cudaStream_t s);
+
 }  // namespace dnb

@@ -168,6 +168,14 @@ extern "C" int dnb_attention_forward(dnb_attention_plan *p, const dnb_tensor *q,
     a.status = p->status; a.wait_limit = p->wait_limit; a.debug = p->debug;
     if (p->device < 0) DNB_FAIL(DNB_ECUDA, "attention: the plan was made without a CUDA device");
     DNB_TRY(check_current_device(p->device, "attention"));
+    if (attention_rows_covers(a, q->dtype)) {
+        p->kernel = "rows_bf16";
+        return launch_attention_rows(a, (cudaStream_t)stream);
+    }
+    if (attention_f32_covers(a, q->dtype)) {
+        p->kernel = "fma_f32";
+        return launch_attention_f32(a, (cudaStream_t)stream);
+    }
     if (attention_tc_covers(a, q->dtype)) {
         p->kernel = "tc_bf16";
         return launch_attention_tc(a, (cudaStream_t)stream);

@@ -1,0 +1,339 @@
+// Cross attention of bf16 tensors for few query rows a key head: single tokens, and the query heads that share its keys.
+//
+// The bytes of keys and values bound it: each is read once, by TMA, through a ring of tiles of 64 keys that keeps about 100 KB an SM's block (two of
+// them an SM) on the way.  Four warps, 16 keys of a tile each, multiply them by up to 16 rows with mma.sync: the 128 rows of a tcgen05 product would be
+// empty but for a few, its TMEM round trip is a latency for each tile, and the arithmetic is far from any bound either way.  A warp has a running maximum
+// and sum of its own keys; warps, and the CTAs of a cluster that share the keys of one head, meet once at the end.
+#include <atomic>
+
+#include "attention.cuh"
+
+namespace dnb {
+
+int encode_tensor_map(CUtensorMap *map, int elem_kind, int rank, void *base, const uint64_t *dims, const uint64_t *strides_bytes, const uint32_t *box, int swizzle_bytes);
+
+namespace {
+
+constexpr int R_KEYS = 64, R_WARPS = 4, R_THREADS = R_WARPS * 32 + 32;
+constexpr float R_MOVE = 8.f;                     // how far (log2) scores may outgrow the running maximum before the sums are corrected
+
+template <int DP> struct RowsCfg {
+    static constexpr int BOXES = DP / 64;
+    static constexpr uint32_t BOX = R_KEYS * 128, TILE = BOXES * BOX;
+    static constexpr int STAGES = DP == 128 ? 6 : 12;
+    static constexpr int PITCH = DP + 4;
+    static constexpr uint32_t WORK = STAGES * TILE;
+    static_assert((R_WARPS + 1) * 16 * PITCH * 4 <= (int)WORK, "the warps' sums fit where the tiles were");
+};
+
+struct RowsShared {
+    uint64_t full[12], empty[12];
+    int abort_flag;
+    float top[R_WARPS * 16], sum[R_WARPS * 16], all_top[16], all_sum[16];
+};
+
+struct alignas(64) RowsArgs {
+    CUtensorMap tmk, tmv;
+    AttnArgs a;
+    int splits;
+    float scale_log2;
+};
+
+__device__ __forceinline__ void ldsm4(uint32_t at, uint32_t (&r)[4])
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t at, uint32_t (&r)[4])
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <int DP>
+__global__ void __launch_bounds__(R_THREADS, 2)
+attention_rows_kernel(const __grid_constant__ RowsArgs t)
+{
+    using C = RowsCfg<DP>;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    const AttnArgs &a = t.a;
+    const uint32_t ring = smem_u32(smem_raw);
+    if (ring & 1023u) {
+        if (threadIdx.x == 0) atomicCAS(a.status, 0, AT_SMEM_BASE);
+        return;
+    }
+    RowsShared *sh = reinterpret_cast<RowsShared *>(smem_raw + C::WORK);
+    volatile int *abort_flag = &sh->abort_flag;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    const int rank = (int)(blockIdx.x % (unsigned)t.splits), job = (int)(blockIdx.x / (unsigned)t.splits);
+    const int kv_head = job % a.kv_heads, image = job / a.kv_heads;
+    const int rows = a.lq * a.group;                                    // row r: token r / group, head r % group of the group
+    if (tid == 0) {
+        for (int i = 0; i < C::STAGES; ++i) {
+            mbar_init(smem_u32(&sh->full[i]), 1);
+            mbar_init(smem_u32(&sh->empty[i]), R_WARPS);
+        }
+        sh->abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncthreads();
+    grid_dependency_wait();
+    launch_dependents_if_small();
+
+    int keys = a.lk, first, tiles;
+    if (a.lengths) keys = min(max(a.lengths[image], 0), a.lk);
+    share_of_keys(keys, R_KEYS, rank, t.splits, first, tiles);
+    // the token and head of row r: where its channels start in q (and, with y's pitch, in y)
+    auto q_at = [&](int r, int pitch) { return ((size_t)image * a.lq + r / a.group) * pitch + (kv_head * a.group + r % a.group) * a.d; };
+
+    if (warp == R_WARPS) {
+        int stage = 0;
+        uint32_t phase = 0;
+        for (int i = 0; i < 2 * tiles; ++i) {
+            const uint32_t full = smem_u32(&sh->full[stage]);
+            if (!mbar_wait_warp(smem_u32(&sh->empty[stage]), phase ^ 1, abort_flag, a.status, AT_SLOT, a.wait_limit)) break;
+            if (elect_one() && !(a.debug & 32 && i == 1)) {
+                mbar_expect_tx(full, C::TILE);
+                for (int b = 0; b < C::BOXES; ++b)
+                    tma_load_4d(ring + stage * C::TILE + b * C::BOX, i & 1 ? &t.tmv : &t.tmk, full, b * 64, kv_head, (first + i / 2) * R_KEYS, a.kn == 1 ? 0 : image);
+            }
+            if (++stage == C::STAGES) { stage = 0; phase ^= 1; }
+        }
+        __syncwarp();
+    }
+
+    const int g = lane >> 2, c2 = (lane & 3) * 2;                       // this lane's rows g and g + 8 of a product, columns c2 and c2 + 1
+    float o[DP / 8][4] = {}, top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+    bool ok = true;
+    if (warp < R_WARPS && tiles > 0) {
+        uint32_t q[DP / 16][4];
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = g + (e & 1) * 8, c = i * 16 + c2 + (e >> 1) * 8;
+                q[i][e] = r < rows && c < a.d ? *reinterpret_cast<const uint32_t *>((const __nv_bfloat16 *)a.q + q_at(r, a.qp) + c) : 0u;
+            }
+        const uint8_t *mask[2] = {nullptr, nullptr};
+        if (a.mask)
+            for (int e = 0; e < 2; ++e) mask[e] = a.mask + (long long)image * a.mask_image + (long long)(g + e * 8 < rows ? (g + e * 8) / a.group : 0) * a.mask_query;
+        const int m = lane >> 3, mr = lane & 7;                         // the 8x8 matrix and its row whose address this lane gives
+        int stage = 0;
+        uint32_t phase = 0;
+        auto next = [&]() { if (++stage == C::STAGES) { stage = 0; phase ^= 1; } };
+        for (int j = 0; j < tiles; ++j) {
+            const int key0 = (first + j) * R_KEYS + warp * 16, left = keys - key0;
+            bool in[2][4];                                              // row e, keys c2, c2 + 1, 8 + c2, 8 + c2 + 1
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int key = (i >> 1) * 8 + c2 + (i & 1);
+                    in[e][i] = key < left && (!a.mask || mask[e][key0 + key]);
+                }
+            if (!mbar_wait(smem_u32(&sh->full[stage]), phase, abort_flag, a.status, AT_KEYS, 0, a.wait_limit)) { ok = false; break; }
+            float s[2][4] = {};
+            {
+                const int key = warp * 16 + (m >> 1) * 8 + mr;
+                const uint32_t at = ring + stage * C::TILE + key * 128;
+#pragma unroll
+                for (int i = 0; i < DP / 16; ++i) {
+                    const int c = i * 16 + (m & 1) * 8;
+                    uint32_t b[4];
+                    ldsm4(at + (c >> 6) * C::BOX + (((c & 63) * 2) ^ (mr << 4)), b);
+                    mma16816(s[0], q[i], b[0], b[1]);
+                    mma16816(s[1], q[i], b[2], b[3]);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sh->empty[stage]));
+            next();
+            float grown[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                grown[e] = top[e];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float &v = s[i >> 1][e * 2 + (i & 1)];
+                    v = in[e][i] ? v * t.scale_log2 : -INFINITY;
+                    grown[e] = fmaxf(grown[e], v);
+                }
+                grown[e] = fmaxf(grown[e], __shfl_xor_sync(0xffffffffu, grown[e], 1));
+                grown[e] = fmaxf(grown[e], __shfl_xor_sync(0xffffffffu, grown[e], 2));
+            }
+            if (__any_sync(0xffffffffu, grown[0] - top[0] > R_MOVE || grown[1] - top[1] > R_MOVE)) {
+                float shrink[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    shrink[e] = grown[e] == top[e] ? 1.f : ex2(top[e] - grown[e]);
+                    top[e] = grown[e];
+                    sum[e] *= shrink[e];
+                }
+#pragma unroll
+                for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[i][e] *= shrink[e >> 1];
+            }
+            uint32_t p[4];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float base = top[e] == -INFINITY ? 0.f : top[e];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float x = ex2(s[i][e * 2] - base), z = ex2(s[i][e * 2 + 1] - base);
+                    sum[e] += x + z;
+                    p[i * 2 + e] = pack_bf16(x, z);
+                }
+            }
+            if (!mbar_wait(smem_u32(&sh->full[stage]), phase, abort_flag, a.status, AT_VALUES, 0, a.wait_limit)) { ok = false; break; }
+            const uint32_t v_tile = stage * C::TILE;
+            if ((left < 16 && keys < a.lk) || (a.mask && a.mask_query == 0)) {
+                // values that no weight reaches may be anything: zeros in their place, this warp's keys by this warp
+                const int key = lane >> 1;
+                if (key >= left || (a.mask && a.mask_query == 0 && !mask[0][key0 + key])) {
+#pragma unroll
+                    for (int b = 0; b < C::BOXES; ++b)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            *reinterpret_cast<uint4 *>(smem_raw + v_tile + b * C::BOX + (warp * 16 + key) * 128 + (lane & 1) * 64 + e * 16) = make_uint4(0, 0, 0, 0);
+                }
+                fence_async_smem();                                     // before the slot's next load
+                __syncwarp();
+            }
+            {
+                const int key = warp * 16 + (m & 1) * 8 + mr;
+                const uint32_t at = ring + v_tile + key * 128;
+#pragma unroll
+                for (int i = 0; i < DP / 16; ++i) {
+                    const int c = i * 16 + (m >> 1) * 8;
+                    uint32_t b[4];
+                    ldsm4t(at + (c >> 6) * C::BOX + (((c & 63) * 2) ^ (mr << 4)), b);
+                    mma16816(o[2 * i], p, b[0], b[1]);
+                    mma16816(o[2 * i + 1], p, b[2], b[3]);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sh->empty[stage]));
+            next();
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 1);
+        sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 2);
+    }
+    __syncthreads();                                                    // every tile has been read: its memory takes the sums
+    float *parts = reinterpret_cast<float *>(smem_raw), *whole = parts + R_WARPS * 16 * C::PITCH;
+    if (warp < R_WARPS) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int r = warp * 16 + g + e * 8;
+            if ((lane & 3) == 0) { sh->top[r] = top[e]; sh->sum[r] = sum[e]; }
+            if (g + e * 8 < rows)
+#pragma unroll
+                for (int i = 0; i < DP / 8; ++i) *reinterpret_cast<float2 *>(parts + r * C::PITCH + i * 8 + c2) = make_float2(o[i][e * 2], o[i][e * 2 + 1]);
+        }
+    }
+    __syncthreads();
+    // the warps' sums to the block's, or to the output where the block has all keys
+    const int chunks = a.d / 4;
+    for (int i = tid; i < rows * chunks && !*abort_flag; i += R_THREADS) {
+        const int r = i / chunks, c = (i - r * chunks) * 4;
+        float most = -INFINITY, total = 0.f;
+#pragma unroll
+        for (int w = 0; w < R_WARPS; ++w) most = fmaxf(most, sh->top[w * 16 + r]);
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < R_WARPS; ++w) {
+            const float l = sh->sum[w * 16 + r], m = sh->top[w * 16 + r];
+            if (l == 0.f) continue;
+            const float f = m == most ? 1.f : ex2(m - most);
+            const float4 z = *reinterpret_cast<const float4 *>(parts + (w * 16 + r) * C::PITCH + c);
+            total += l * f;
+            x.x = fmaf(z.x, f, x.x); x.y = fmaf(z.y, f, x.y); x.z = fmaf(z.z, f, x.z); x.w = fmaf(z.w, f, x.w);
+        }
+        if (t.splits == 1) {
+            const float inv = total == 0.f ? 0.f : 1.f / total;
+            *reinterpret_cast<uint2 *>((__nv_bfloat16 *)a.y + q_at(r, a.yp) + c) = make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
+        } else {
+            *reinterpret_cast<float4 *>(whole + r * C::PITCH + c) = x;
+            if (c == 0) { sh->all_top[r] = most; sh->all_sum[r] = total; }
+        }
+    }
+    if (t.splits > 1) {
+        __syncwarp();
+        cluster_sync_all();
+        if (!*abort_flag)
+            join_rows<__nv_bfloat16>(smem_u32(whole), C::PITCH, smem_u32(sh->all_top), smem_u32(sh->all_sum), rows, a.d, rank, t.splits, tid, R_THREADS,
+                                     [&](int r) { return (__nv_bfloat16 *)a.y + q_at(r, a.yp); });
+        __syncwarp();
+        cluster_sync_all();
+    }
+    if (*abort_flag) {                                                  // loads in flight land before their memory goes
+        const long long begin = clock64();
+        while (clock64() - begin < 4000000LL) { }
+    }
+    (void)ok;
+}
+
+typedef void (*RowsKernel)(RowsArgs);
+
+}  // namespace
+
+bool attention_rows_covers(const AttnArgs &a, int dtype)
+{
+    return dtype == DNB_BF16 && a.d <= 128 && (long long)a.lq * a.group <= 16 && (long long)a.n * a.kv_heads < 1LL << 28;
+}
+
+int launch_attention_rows(const AttnArgs &a, cudaStream_t stream)
+{
+    RowsArgs t;
+    t.a = a;
+    if (!t.a.wait_limit) t.a.wait_limit = WAIT_LIMIT_CYCLES;
+    t.scale_log2 = a.scale * 1.4426950408889634f;
+    auto map = [&](CUtensorMap *m, const void *data, int pitch) {
+        const uint64_t dims[4] = {(uint64_t)a.d, (uint64_t)a.kv_heads, (uint64_t)a.lk, (uint64_t)a.kn};
+        const uint64_t strides[3] = {(uint64_t)a.d * 2, (uint64_t)pitch * 2, (uint64_t)a.lk * pitch * 2};
+        const uint32_t box[4] = {64, 1, R_KEYS, 1};
+        return encode_tensor_map(m, 1, 4, const_cast<void *>(data), dims, strides, box, 128);
+    };
+    DNB_TRY(map(&t.tmk, a.k, a.kp));
+    DNB_TRY(map(&t.tmv, a.v, a.vp));
+    // Two blocks an SM: split the keys while there is room for twice the blocks, a tile a block at least.
+    const long long jobs = (long long)a.n * a.kv_heads;
+    const int key_tiles = (a.lk + R_KEYS - 1) / R_KEYS;
+    t.splits = 1;
+    while (t.splits < 8 && jobs * t.splits * 2 <= 2 * sm_count() && key_tiles >= t.splits * 2) t.splits *= 2;
+    const bool big = a.d > 64;
+    const RowsKernel kern = big ? attention_rows_kernel<128> : attention_rows_kernel<64>;
+    const size_t bytes = (big ? RowsCfg<128>::WORK : RowsCfg<64>::WORK) + sizeof(RowsShared);
+    static std::atomic<bool> done[64][2];
+    int dev = 0;
+    DNB_CUDA(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64) DNB_FAIL(DNB_ECUDA, "attention: device %d", dev);
+    if (!done[dev][big].load(std::memory_order_acquire)) {
+        DNB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+        done[dev][big].store(true, std::memory_order_release);
+    }
+    cudaLaunchAttribute attrs[2];
+    attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[0].val.programmaticStreamSerializationAllowed = pdl_enabled() && jobs * t.splits <= EARLY_BLOCKS ? 1 : 0;
+    attrs[1].id = cudaLaunchAttributeClusterDimension;
+    attrs[1].val.clusterDim.x = (unsigned)t.splits; attrs[1].val.clusterDim.y = 1; attrs[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(jobs * t.splits));
+    cfg.blockDim = dim3(R_THREADS);
+    cfg.dynamicSmemBytes = bytes;
+    cfg.stream = stream;
+    cfg.attrs = attrs;
+    cfg.numAttrs = 2;
+    DNB_CUDA(cudaLaunchKernelEx(&cfg, kern, t));
+    DNB_LAUNCH_CHECK("attention");
+    return DNB_OK;
+}
+
+}  // namespace dnb

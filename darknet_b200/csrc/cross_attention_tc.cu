@@ -16,9 +16,7 @@
 // workspace, one launch, the same order of additions every time.
 #include <atomic>
 
-#include "attention.h"
-#include "device_utils.cuh"
-#include "tc_ptx.cuh"
+#include "attention.cuh"
 
 namespace dnb {
 
@@ -32,8 +30,6 @@ constexpr int THREADS = 320;                      // two warpgroups of softmax, 
 constexpr int MAX_STAGES = 12;
 constexpr uint32_t BOX_BYTES = 128 * 128;         // 64 channels of 128 rows
 constexpr float MOVE = 8.f;                       // how far (log2) scores may outgrow the running maximum
-
-enum { AT_QUERIES = 201, AT_SLOT, AT_KEYS, AT_VALUES, AT_SCORES, AT_WEIGHTS, AT_OUTPUT, AT_SMEM_BASE };
 
 struct Shared {
     uint64_t q_full, full[MAX_STAGES], empty[MAX_STAGES], s_full[2], p_full[2], o_full[2];
@@ -71,19 +67,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-__device__ __forceinline__ float ex2(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi)
-{
-    uint32_t r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-
 // 32 columns of this warp's 32 lanes
 __device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t *r)
 {
@@ -122,23 +105,6 @@ __device__ __forceinline__ void umma_from_tmem(uint32_t tmem_d, uint32_t tmem_a,
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
         ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
 }
-__device__ __forceinline__ float4 ld_peer(uint32_t addr, uint32_t rank)
-{
-    float4 v;
-    asm volatile(
-        "{\n\t.reg .b32 at;\n\t"
-        "mapa.shared::cluster.u32 at, %4, %5;\n\t"
-        "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [at];\n\t}"
-        : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr), "r"(rank) : "memory");
-    return v;
-}
-__device__ __forceinline__ float ld_peer1(uint32_t addr, uint32_t rank)
-{
-    float v;
-    asm volatile("{\n\t.reg .b32 at;\n\tmapa.shared::cluster.u32 at, %1, %2;\n\tld.shared::cluster.f32 %0, [at];\n\t}" : "=f"(v) : "r"(addr), "r"(rank) : "memory");
-    return v;
-}
-
 // DP: channels of a head as they lie in shared memory, 64 or 128 (TMA fills what the head does not have with zeros).
 template <int DP> struct Cfg {
     static constexpr int BOXES = DP / 64;
@@ -202,8 +168,8 @@ attention_tc_kernel(const __grid_constant__ TcAttnArgs t)
 
     int keys = a.lk;
     if (a.lengths) keys = min(max(a.lengths[image], 0), a.lk);
-    const int all = (keys + 127) >> 7, per = (all + t.splits - 1) / t.splits;
-    const int t0 = min(rank * per, all), tiles = min(t0 + per, all) - t0;
+    int t0, tiles;
+    share_of_keys(keys, 128, rank, t.splits, t0, tiles);
 
     if (warp == 8) {
         // ---------------------------------------------------------------- loads
@@ -432,7 +398,7 @@ attention_tc_kernel(const __grid_constant__ TcAttnArgs t)
         __syncthreads();                                                // the other tile's products have read their operands too
         float *rows = reinterpret_cast<float *>(smem_raw);
         if (mine) {
-            sh->top[s * 128 + row] = top;
+            sh->top[s * 128 + row] = top * t.scale_log2;
             sh->sum[s * 128 + row] = sum;
             if (tiles > 0 && ok) {
 #pragma unroll 1
@@ -447,38 +413,13 @@ attention_tc_kernel(const __grid_constant__ TcAttnArgs t)
             }
         }
         cluster_sync_all();
-        // Rows rank, rank + splits, ... of the pair of tiles, `splits` threads a row: the shares' sums, in the order of the keys.
-        if (tid < 128 * sides && !*abort_flag) {
-            const int part = tid % t.splits, r = tid / t.splits * t.splits + rank, side = r >> 7, in_tile = r & 127;
-            const int token = token0 + side * t.q_tokens + in_tile / a.group;
-            if (in_tile < t.q_tokens * a.group && token < a.lq) {
-                float most = -INFINITY, weight[8], total = 0.f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (i < t.splits) most = fmaxf(most, ld_peer1(smem_u32(&sh->top[r]), i));
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (i < t.splits) {
-                        const float m = ld_peer1(smem_u32(&sh->top[r]), i), l = ld_peer1(smem_u32(&sh->sum[r]), i);
-                        weight[i] = l == 0.f ? 0.f : m == most ? 1.f : ex2((m - most) * t.scale_log2);   // no weights: its rows hold nothing
-                        total += l * weight[i];
-                    }
-                const float inv = total == 0.f ? 0.f : 1.f / total;
-                __nv_bfloat16 *out = (__nv_bfloat16 *)a.y + ((size_t)image * a.lq + token) * a.yp + (kv_head * a.group + in_tile % a.group) * a.d;
-                for (int c = part * 8; c < a.d; c += t.splits * 8) {
-                    float o[8] = {};
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (i < t.splits && weight[i] != 0.f) {
-                            const float4 x = ld_peer(smem_u32(rows + r * C::PITCH + c), i), z = ld_peer(smem_u32(rows + r * C::PITCH + c + 4), i);
-                            o[0] = fmaf(x.x, weight[i], o[0]); o[1] = fmaf(x.y, weight[i], o[1]); o[2] = fmaf(x.z, weight[i], o[2]); o[3] = fmaf(x.w, weight[i], o[3]);
-                            o[4] = fmaf(z.x, weight[i], o[4]); o[5] = fmaf(z.y, weight[i], o[5]); o[6] = fmaf(z.z, weight[i], o[6]); o[7] = fmaf(z.w, weight[i], o[7]);
-                        }
-                    *reinterpret_cast<uint4 *>(out + c) = make_uint4(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv),
-                                                                     pack_bf16(o[4] * inv, o[5] * inv), pack_bf16(o[6] * inv, o[7] * inv));
-                }
-            }
-        }
+        if (!*abort_flag)
+            join_rows<__nv_bfloat16>(smem_u32(rows), C::PITCH, smem_u32(sh->top), smem_u32(sh->sum), 128 * sides, a.d, rank, t.splits, tid, THREADS, [&](int r) -> __nv_bfloat16 * {
+                const int in_tile = r & 127, token = token0 + (r >> 7) * t.q_tokens + in_tile / a.group;
+                if (in_tile >= t.q_tokens * a.group || token >= a.lq) return nullptr;
+                return (__nv_bfloat16 *)a.y + ((size_t)image * a.lq + token) * a.yp + (kv_head * a.group + in_tile % a.group) * a.d;
+            });
+        __syncwarp();
         cluster_sync_all();                                             // a peer's rows are read until here
     }
     if (*abort_flag) {                                                  // loads and products in flight end before their memory goes
