@@ -20,124 +20,185 @@ struct NormArgs {
     float *scales;
     long long tokens;
     int c, xp, rp, sp, yp, qp;
-    int group, groups;      // channels that share a scale, and how many scales a token has
+    int group, group_log2;  // channels that share a scale
+    int groups;             // scales of a token
     float eps;
 };
 
-constexpr int NORM_VECS = 4;        // 16-byte vectors a thread holds of one token
+constexpr int NORM_VECS = 4;        // 16-byte vectors a thread holds of one token, at most
 constexpr int NORM_MAX_WARPS = 32;  // warps of one token
 
-// max that a NaN wins, so that a token with one says so in its scale
-__device__ __forceinline__ float max_nan(float a, float b)
+// Two values of a 16-byte vector at a time, as floats.
+template <typename T> struct Pairs;
+template <> struct Pairs<float> {
+    static constexpr int N = 2;
+    static __device__ __forceinline__ void get(uint4 v, uint64_t *o)
+    {
+        o[0] = pack2(__uint_as_float(v.x), __uint_as_float(v.y));
+        o[1] = pack2(__uint_as_float(v.z), __uint_as_float(v.w));
+    }
+    static __device__ __forceinline__ uint4 put(const uint64_t *v)
+    {
+        float x[4];
+        unpack2(v[0], x[0], x[1]);
+        unpack2(v[1], x[2], x[3]);
+        return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+    }
+};
+template <> struct Pairs<__nv_bfloat16> {
+    static constexpr int N = 4;
+    static __device__ __forceinline__ void get(uint4 v, uint64_t *o)
+    {
+        o[0] = bf16_pair(v.x);
+        o[1] = bf16_pair(v.y);
+        o[2] = bf16_pair(v.z);
+        o[3] = bf16_pair(v.w);
+    }
+    static __device__ __forceinline__ uint4 put(const uint64_t *v) { return make_uint4(pack_bf16(v[0]), pack_bf16(v[1]), pack_bf16(v[2]), pack_bf16(v[3])); }
+};
+
+// The larger of |v|'s two and `most`, as integers: magnitudes of floats are ordered like them, and a NaN is above infinity, so that a token with one says
+// so in its scale.
+__device__ __forceinline__ uint32_t larger_magnitude(uint64_t v, uint32_t most)
 {
-    float m;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
-    return m;
+    float a, b;
+    unpack2(v, a, b);
+    return __vimax3_u32(__float_as_uint(a) & 0x7fffffffu, __float_as_uint(b) & 0x7fffffffu, most);
 }
 
-// WARPS warps a token, several tokens a block where that is one.
-template <typename T, int WARPS>
-__global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32)
+// WARPS warps a token (four tokens a block where that is one), VECS 16-byte vectors a thread.  A thread meets the same channels in every token: it keeps
+// their gains.  Q: the output in 8 bits.  WHOLE: a token's channels are as many as its threads hold, so that nothing is cut off.
+template <typename T, int WARPS, int VECS, bool Q, bool WHOLE>
+__global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32, WARPS > 4 ? 1 : VECS <= 2 ? 8 : 5)
 rmsnorm_kernel(const __grid_constant__ NormArgs a)
 {
+    using P = Pairs<T>;
     constexpr int N = 16 / sizeof(T), ROWS = WARPS == 1 ? 4 : 1, LANES = WARPS * 32;
-    union Vec { uint4 raw; T v[N]; };
-    __shared__ float part[2][NORM_MAX_WARPS];
-    grid_dependency_wait();
-    launch_dependents_if_small();
+    __shared__ float part[NORM_MAX_WARPS];
+    __shared__ uint32_t tops[NORM_MAX_WARPS];
     const int lane = WARPS == 1 ? threadIdx.x & 31 : threadIdx.x, warp = threadIdx.x >> 5;
     const int vecs = (a.c + 7) / 8 * 8 / N;
-    for (long long token = (long long)blockIdx.x * ROWS + (WARPS == 1 ? warp : 0); token < a.tokens; token += (long long)gridDim.x * ROWS) {
-        float v[NORM_VECS][N];
-        float squares = 0.f;
+    grid_dependency_wait();
+    launch_dependents_if_small();
+    const float per_channel = 1.f / (float)a.c;
+    uint64_t gain[VECS][P::N];
 #pragma unroll
-        for (int k = 0; k < NORM_VECS; ++k) {
-            const int at = lane + k * LANES;
-            if (at >= vecs) break;
-            Vec x, r;
-            x.raw = reinterpret_cast<const uint4 *>((const T *)a.x + (size_t)token * a.xp)[at];
-            if (a.r) r.raw = reinterpret_cast<const uint4 *>((const T *)a.r + (size_t)token * a.rp)[at];
+    for (int k = 0; k < VECS; ++k)
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-                v[k][e] = to_float<T>(x.v[e]);
-                if (a.r) v[k][e] += to_float<T>(r.v[e]);
-                if (at * N + e >= a.c) v[k][e] = 0.f;       // padding channels
-            }
-            if (a.sum) {
-                Vec o;
-#pragma unroll
-                for (int e = 0; e < N; ++e) o.v[e] = from_float<T>(v[k][e]);
-                reinterpret_cast<uint4 *>((T *)a.sum + (size_t)token * a.sp)[at] = o.raw;
-            }
-#pragma unroll
-            for (int e = 0; e < N; ++e) squares = fmaf(v[k][e], v[k][e], squares);
+        for (int e = 0; e < P::N; ++e) {
+            const int ch = (lane + k * LANES) * N + 2 * e;
+            gain[k][e] = pack2(a.gain && ch < a.c ? __ldg(a.gain + ch) : 1.f, a.gain && ch + 1 < a.c ? __ldg(a.gain + ch + 1) : 1.f);
         }
+    // zeros in the place of padding channels, and of what lies behind them
+    auto cut = [&](uint64_t *v, int at) {
+        if constexpr (!WHOLE) {
+            if (at * N + N <= a.c) return;
+#pragma unroll
+            for (int e = 0; e < P::N; ++e) {
+                float lo, hi;
+                unpack2(v[e], lo, hi);
+                v[e] = pack2(at * N + 2 * e < a.c ? lo : 0.f, at * N + 2 * e + 1 < a.c ? hi : 0.f);
+            }
+        }
+    };
+    auto holds = [&](int at) { return WHOLE || at < vecs; };
+    long long token = (long long)blockIdx.x * ROWS + (WARPS == 1 ? warp : 0);
+    const long long step = (long long)gridDim.x * ROWS;
+    const T *px = (const T *)a.x + token * a.xp + lane * N, *pr = (const T *)a.r + token * a.rp + lane * N;
+    T *ps = (T *)a.sum + token * a.sp + lane * N, *py = (T *)a.y + token * a.yp + lane * N;
+    uint8_t *pq = a.q + token * a.qp + lane * N;
+    float *pscale = a.scales + token * a.groups;
+    for (; token < a.tokens; token += step, px += step * a.xp, pr += step * a.rp, ps += step * a.sp, py += step * a.yp, pq += step * a.qp, pscale += step * a.groups) {
+        uint4 x[VECS], r[VECS];
+#pragma unroll
+        for (int k = 0; k < VECS; ++k) {                    // all loads of a token in flight together
+            x[k] = r[k] = make_uint4(0, 0, 0, 0);
+            if (holds(lane + k * LANES)) {
+                x[k] = *reinterpret_cast<const uint4 *>(px + k * LANES * N);
+                if (a.r) r[k] = *reinterpret_cast<const uint4 *>(pr + k * LANES * N);
+            }
+        }
+        uint64_t v[VECS][P::N], squares2[2] = {0, 0};
+#pragma unroll
+        for (int k = 0; k < VECS; ++k) {
+            const int at = lane + k * LANES;
+            uint64_t t[P::N];
+            P::get(x[k], v[k]);
+            P::get(r[k], t);
+#pragma unroll
+            for (int e = 0; e < P::N; ++e) v[k][e] = add2(v[k][e], t[e]);       // without a residual: zeros
+            cut(v[k], at);
+#pragma unroll
+            for (int e = 0; e < P::N; ++e) squares2[e & 1] = fma2(v[k][e], v[k][e], squares2[e & 1]);
+            if (a.sum && holds(at)) *reinterpret_cast<uint4 *>(ps + k * LANES * N) = P::put(v[k]);
+        }
+        float squares, odd;
+        unpack2(add2(squares2[0], squares2[1]), squares, odd);
+        squares += odd;
 #pragma unroll
         for (int o = 16; o; o >>= 1) squares += __shfl_xor_sync(0xffffffffu, squares, o);
         if (WARPS > 1) {
-            if ((threadIdx.x & 31) == 0) part[0][warp] = squares;
+            if ((threadIdx.x & 31) == 0) part[warp] = squares;
             __syncthreads();
-            squares = part[0][0];
-            for (int i = 1; i < WARPS; ++i) squares += part[0][i];
+            squares = part[0];
+            for (int i = 1; i < WARPS; ++i) squares += part[i];
         }
-        const float inv = 1.f / sqrtf(squares / (float)a.c + a.eps);
-        float most = 0.f;
+        const float inv = rsqrtf(fmaf(squares, per_channel, a.eps));
+        const uint64_t inv2 = pack2(inv, inv);
+        uint32_t most = 0;
 #pragma unroll
-        for (int k = 0; k < NORM_VECS; ++k) {
+        for (int k = 0; k < VECS; ++k) {
             const int at = lane + k * LANES;
-            if (at >= vecs) break;
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-                const int ch = at * N + e;
-                v[k][e] *= inv;
-                if (a.gain && ch < a.c) v[k][e] *= __ldg(a.gain + ch);
-                if (ch >= a.c) v[k][e] = 0.f;               // ... of a token whose inv is no number
-                most = max_nan(most, fabsf(v[k][e]));
-            }
-            if (a.y) {
-                Vec o;
+            for (int e = 0; e < P::N; ++e) v[k][e] = mul2(mul2(v[k][e], inv2), gain[k][e]);
+            cut(v[k], at);                                  // ... of a token whose inv is no number
+            if (Q && !a.group)
 #pragma unroll
-                for (int e = 0; e < N; ++e) o.v[e] = from_float<T>(v[k][e]);
-                reinterpret_cast<uint4 *>((T *)a.y + (size_t)token * a.yp)[at] = o.raw;
-            }
+                for (int e = 0; e < P::N; ++e) most = larger_magnitude(v[k][e], most);
+            if (a.y && holds(at)) *reinterpret_cast<uint4 *>(py + k * LANES * N) = P::put(v[k]);
         }
-        if (a.q) {
+        if (Q) {
             if (!a.group) {
-#pragma unroll
-                for (int o = 16; o; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+                most = __reduce_max_sync(0xffffffffu, most);
                 if (WARPS > 1) {
-                    if ((threadIdx.x & 31) == 0) part[1][warp] = most;
+                    if ((threadIdx.x & 31) == 0) tops[warp] = most;
                     __syncthreads();
-                    most = part[1][0];
-                    for (int i = 1; i < WARPS; ++i) most = max_nan(most, part[1][i]);
+                    most = tops[0];
+                    for (int i = 1; i < WARPS; ++i) most = max(most, tops[i]);
                 }
             }
 #pragma unroll
-            for (int k = 0; k < NORM_VECS; ++k) {
+            for (int k = 0; k < VECS; ++k) {                // every lane of a group is here for the shuffles, whether it holds channels or not
                 const int at = lane + k * LANES;
-                if (k * LANES >= vecs) break;               // by whole rounds: the lanes of a group meet in the shuffles
                 if (a.group) {
-                    most = 0.f;
-                    if (at < vecs)
+                    most = 0;
 #pragma unroll
-                        for (int e = 0; e < N; ++e) most = max_nan(most, fabsf(v[k][e]));
-                    for (int o = a.group / N / 2; o; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+                    for (int e = 0; e < P::N; ++e) most = larger_magnitude(v[k][e], most);
+#pragma unroll
+                    for (int o = 1; o < 32; o *= 2)
+                        if (o * N < a.group) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
                 }
-                if (at >= vecs) continue;
-                const float scale = max_nan(most / 448.f, 0x1p-126f);
-                const int g = a.group ? at * N / a.group : 0;
-                if (a.group ? at * N % a.group == 0 : at == 0) a.scales[(size_t)token * a.groups + g] = scale;
+                if (!holds(at)) continue;
+                // Times the scale's reciprocal, not over the scale: off by an ulp of fp32 or two, where e4m3's half step is 2^-4.
+                const float scaled = __uint_as_float(most) * (1.f / 448.f);
+                const float scale = scaled < 0x1p-126f ? 0x1p-126f : scaled;    // a NaN stays one
+                float to_q;
+                asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(to_q) : "f"(scale));
+                if (a.group ? (at * N & (a.group - 1)) == 0 : at == 0) pscale[a.group ? at * N >> a.group_log2 : 0] = scale;
+                const uint64_t to_q2 = pack2(to_q, to_q);
                 uint32_t out[N / 4];
 #pragma unroll
-                for (int e = 0; e < N; e += 4) {
-                    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[k][e] / scale, v[k][e + 1] / scale), __NV_SATFINITE, __NV_E4M3);
-                    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[k][e + 2] / scale, v[k][e + 3] / scale), __NV_SATFINITE, __NV_E4M3);
-                    out[e / 4] = lo | hi << 16;
+                for (int e = 0; e < P::N; e += 2) {
+                    float2 lo, hi;
+                    unpack2(mul2(v[k][e], to_q2), lo.x, lo.y);
+                    unpack2(mul2(v[k][e + 1], to_q2), hi.x, hi.y);
+                    out[e / 2] = (uint32_t)__nv_cvt_float2_to_fp8x2(lo, __NV_SATFINITE, __NV_E4M3) | (uint32_t)__nv_cvt_float2_to_fp8x2(hi, __NV_SATFINITE, __NV_E4M3) << 16;
                 }
+                if (!WHOLE && at * N + N > a.c)             // the padding of a token whose scale is no number is zero all the same
 #pragma unroll
-                for (int e = 0; e < N; ++e)                 // the padding of a token whose scale is no number is zero all the same
-                    if (at * N + e >= a.c) out[e / 4] &= ~(0xffu << e % 4 * 8);
-                uint8_t *to = a.q + (size_t)token * a.qp + at * N;
+                    for (int e = 0; e < N; ++e)
+                        if (at * N + e >= a.c) out[e / 4] &= ~(0xffu << e % 4 * 8);
+                uint8_t *to = pq + k * LANES * N;
                 if constexpr (N == 8) *reinterpret_cast<uint2 *>(to) = make_uint2(out[0], out[1]);
                 else *reinterpret_cast<uint32_t *>(to) = out[0];
             }
@@ -146,17 +207,27 @@ rmsnorm_kernel(const __grid_constant__ NormArgs a)
     }
 }
 
-template <typename T>
-static cudaError_t start_rmsnorm(const NormArgs &a, int warps, cudaStream_t s)
+template <typename T, int WARPS, int VECS>
+static cudaError_t start_rmsnorm(const NormArgs &a, cudaStream_t s)
 {
-    const long long cap = (long long)sm_count() * (warps == 1 ? 16 : 64 / warps), blocks = warps == 1 ? (a.tokens + 3) / 4 : a.tokens;
-    const int grid = (int)(blocks < cap ? blocks : cap);
-    switch (warps) {
-    case 1: return launch_overlapped(rmsnorm_kernel<T, 1>, grid, 128, 0, s, a);
-    case 4: return launch_overlapped(rmsnorm_kernel<T, 4>, grid, 128, 0, s, a);
-    case 8: return launch_overlapped(rmsnorm_kernel<T, 8>, grid, 256, 0, s, a);
-    default: return launch_overlapped(rmsnorm_kernel<T, 32>, grid, 1024, 0, s, a);
-    }
+    const long long cap = (long long)sm_count() * (WARPS == 1 ? 8 : 32 / WARPS), blocks = WARPS == 1 ? (a.tokens + 3) / 4 : a.tokens;
+    const int grid = (int)(blocks < cap ? blocks : cap), threads = WARPS == 1 ? 128 : WARPS * 32;
+    const bool whole = a.c == WARPS * 32 * VECS * (16 / (int)sizeof(T));
+    if (a.q) return whole ? launch_overlapped(rmsnorm_kernel<T, WARPS, VECS, true, true>, grid, threads, 0, s, a) : launch_overlapped(rmsnorm_kernel<T, WARPS, VECS, true, false>, grid, threads, 0, s, a);
+    return whole ? launch_overlapped(rmsnorm_kernel<T, WARPS, VECS, false, true>, grid, threads, 0, s, a) : launch_overlapped(rmsnorm_kernel<T, WARPS, VECS, false, false>, grid, threads, 0, s, a);
+}
+
+// A warp a token while that is enough of it to hold (no barrier), the fewest vectors a thread that hold a token.
+template <typename T>
+static cudaError_t choose_rmsnorm(const NormArgs &a, int vecs, cudaStream_t s)
+{
+    if (vecs <= 32) return start_rmsnorm<T, 1, 1>(a, s);
+    if (vecs <= 64) return start_rmsnorm<T, 1, 2>(a, s);
+    if (vecs <= 128) return start_rmsnorm<T, 1, 4>(a, s);
+    if (vecs <= 4 * 64) return start_rmsnorm<T, 4, 2>(a, s);
+    if (vecs <= 4 * 128) return start_rmsnorm<T, 4, 4>(a, s);
+    if (vecs <= 8 * 128) return start_rmsnorm<T, 8, 4>(a, s);
+    return start_rmsnorm<T, 32, 4>(a, s);
 }
 
 // A tensor of the norm: channels-last with x's extents and dtype; one that is x's own memory has its pitch too.
@@ -197,18 +268,18 @@ extern "C" int dnb_rmsnorm_forward(const dnb_tensor *x, const dnb_tensor *residu
         for (const dnb_tensor *t : {x, residual, sum, y})
             if (t && (t->data == q->data || t->data == (void *)q->scales)) DNB_FAIL(DNB_EINVAL, "rmsnorm: the e4m3 output is another tensor's memory");
         a.q = (uint8_t *)q->data; a.scales = q->scales; a.qp = q->pitch; a.group = q->group;
+        while (a.group >> a.group_log2 > 1) ++a.group_log2;
         a.groups = q->group ? (x->c + q->group - 1) / q->group : 1;
     }
-    const int per_vec = x->dtype == DNB_BF16 ? 8 : 4, vecs = round_up(x->c, 8) / per_vec, need = (vecs + 32 * NORM_VECS - 1) / (32 * NORM_VECS);
-    if (need > NORM_MAX_WARPS) DNB_FAIL(DNB_EUNSUPPORTED, "rmsnorm: %d channels (at most %d of this dtype)", x->c, NORM_MAX_WARPS * 32 * NORM_VECS * per_vec);
+    const int per_vec = x->dtype == DNB_BF16 ? 8 : 4, vecs = round_up(x->c, 8) / per_vec;
+    if (vecs > NORM_MAX_WARPS * 32 * NORM_VECS) DNB_FAIL(DNB_EUNSUPPORTED, "rmsnorm: %d channels (at most %d of this dtype)", x->c, NORM_MAX_WARPS * 32 * NORM_VECS * per_vec);
     a.x = x->data; a.xp = x->cpitch;
     if (residual) { a.r = residual->data; a.rp = residual->cpitch; }
     if (sum) { a.sum = sum->data; a.sp = sum->cpitch; }
     if (y) { a.y = y->data; a.yp = y->cpitch; }
     a.gain = gain; a.eps = eps; a.c = x->c;
     a.tokens = (long long)x->n * x->h * x->w;
-    const int warps = need == 1 ? 1 : need <= 4 ? 4 : need <= 8 ? 8 : 32;
-    DNB_CUDA(x->dtype == DNB_BF16 ? start_rmsnorm<__nv_bfloat16>(a, warps, (cudaStream_t)stream) : start_rmsnorm<float>(a, warps, (cudaStream_t)stream));
+    DNB_CUDA(x->dtype == DNB_BF16 ? choose_rmsnorm<__nv_bfloat16>(a, vecs, (cudaStream_t)stream) : choose_rmsnorm<float>(a, vecs, (cudaStream_t)stream));
     DNB_LAUNCH_CHECK("rmsnorm");
     return DNB_OK;
 }

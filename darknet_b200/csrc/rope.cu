@@ -1,11 +1,10 @@
 // Rotary positions with up to three axes (time, row, column) over channels-last tensors.
 //
 // A pair (a, b) of a head's channels becomes (a cos t - b sin t, a sin t + b cos t) with t = position * scale * frequency of the axis it belongs to.
-// The bytes bound it: every channel is read and written once, and a token's sines are computed once for all of its heads (a table in shared
-// memory), not once per element.
+// The bytes bound it: every channel is read and written once, and a thread works its sines out once for several heads.
 //
 // Angles: sine and cosine want t modulo a turn.  A float of t loses that for far positions (position 1e5 has 1/128 of a radian between neighbours),
-// so the table entry is position * F modulo 2^64, where F is the pair's scale * frequency / 2 pi, its whole turns dropped, in units of 2^-64 turns:
+// so the angle is position * F modulo 2^64, where F is the pair's scale * frequency / 2 pi, its whole turns dropped, in units of 2^-64 turns:
 // one integer product, exact modulo a turn, off by at most position * 2^-65 turns however far the position is.
 #include <math.h>
 #include <string.h>
@@ -25,8 +24,7 @@ struct dnb_rope_plan {
 
 namespace dnb {
 
-constexpr int ROPE_THREADS = 256;
-constexpr int ROPE_TABLE = 2048;           // sines and cosines that a block holds: 16 KB
+constexpr int ROPE_THREADS = 128;
 
 struct RopeArgs {
     uint64_t turn[DNB_ROPE_MAX_PAIRS];
@@ -34,12 +32,13 @@ struct RopeArgs {
     const void *x;
     void *y;
     const int32_t *positions;              // [tokens][3], or null: the token's place
-    long long tokens;
+    unsigned tokens;
     int xp, yp;                            // pitches
     int c, c8;                             // channels, and rounded up to whole vectors of eight
     int h, w, frames, origin[3];
     int heads, head_dim, pairs;
-    int tile;                              // tokens whose table a block holds at a time
+    int chunk, chunks;                     // heads of a thread, and how many such shares a token has
+    unsigned turners;                      // blocks that turn; the blocks behind them copy what passes
 };
 
 template <int BYTES> struct RopeVec;
@@ -48,97 +47,112 @@ template <> struct RopeVec<4> { using type = uint32_t; };
 template <> struct RopeVec<8> { using type = uint2; };
 template <> struct RopeVec<16> { using type = uint4; };
 
-// V pairs an item: V elements at each of two places, in one load each.
+// A thread turns V pairs (V elements at each of two places, a load each) of `chunk` heads of a token; their sines it works out once, in registers.  The
+// threads of a warp lie along the pairs of a head, then along shares of heads, then tokens: loads of 16 bytes fill whole sectors.
 template <typename T, int V, bool INTERLEAVED>
 __global__ void __launch_bounds__(ROPE_THREADS)
 rope_kernel(const __grid_constant__ RopeArgs a)
 {
     using Raw = typename RopeVec<V * (int)sizeof(T)>::type;
     union Vec { Raw raw; T v[V]; };
-    __shared__ float2 table[ROPE_TABLE];
+    constexpr int AT_ONCE = 4;                                                    // heads whose loads are in flight together
     grid_dependency_wait();
     launch_dependents_if_small();
     const T *x = (const T *)a.x;
     T *y = (T *)a.y;
-    const bool copies = a.x != a.y;
-    const int per_head = a.pairs / V, per_token = a.heads * per_head;
-    const int rest = (a.head_dim - 2 * a.pairs) / V;                              // vectors of a head that do not turn
-    const int tail0 = a.heads * a.head_dim, tail = (a.c8 - tail0) / 8;            // channels behind the heads, by eights
-    const long long tiles = (a.tokens + a.tile - 1) / a.tile;
-    for (long long t = blockIdx.x; t < tiles; t += gridDim.x) {
-        const long long first = t * a.tile;
-        const int count = (int)(a.tokens - first < a.tile ? a.tokens - first : a.tile);
-        __syncthreads();                                                          // the last tile's table has been read
-        for (int i = threadIdx.x; i < count * a.pairs; i += ROPE_THREADS) {
-            const int k = i / a.pairs, pair = i - k * a.pairs, axis = a.axis[pair];
-            const long long token = first + k;
-            long long at;
-            if (a.positions) at = a.positions[token * 3 + axis];
-            else {
-                const int row = (int)(token / a.w);
-                at = axis == 2 ? token - (long long)row * a.w : axis == 1 ? row % a.h : row / a.h % a.frames;
-                at += a.origin[axis];
-            }
-            const int turns = (int)((uint64_t)at * a.turn[pair] >> 32);           // signed: from -1/2 to 1/2 of a turn, in units of 2^-32
-            float s, c;
-            sincospif((float)turns * 0x1p-31f, &s, &c);
-            table[i] = make_float2(c, s);
-        }
+    const int per_head = a.pairs / V;
+    if (blockIdx.x < a.turners) {
+        __shared__ uint64_t turn[DNB_ROPE_MAX_PAIRS];                             // threads read them in many orders, constants in one
+        __shared__ uint8_t axis[DNB_ROPE_MAX_PAIRS];
+        for (int i = threadIdx.x; i < a.pairs; i += ROPE_THREADS) { turn[i] = a.turn[i]; axis[i] = a.axis[i]; }
         __syncthreads();
-        for (int i = threadIdx.x; i < count * per_token; i += ROPE_THREADS) {
-            const int k = i / per_token, r = i - k * per_token;
-            const int head = r / per_head, j = (r - head * per_head) * V;
-            const int at_a = head * a.head_dim + (INTERLEAVED ? 2 * j : j), at_b = at_a + (INTERLEAVED ? V : a.pairs);
-            const T *src = x + (size_t)(first + k) * a.xp;
-            T *dst = y + (size_t)(first + k) * a.yp;
-            Vec va, vb;
-            va.raw = *reinterpret_cast<const Raw *>(src + at_a);
-            vb.raw = *reinterpret_cast<const Raw *>(src + at_b);
-            const float2 *cs = table + k * a.pairs + j;
+        const unsigned long long item = (unsigned long long)blockIdx.x * ROPE_THREADS + threadIdx.x;
+        const unsigned part = (unsigned)(item / (unsigned)per_head);              // fits: tokens * chunks < 2^31
+        const int j = (int)(item - (unsigned long long)part * (unsigned)per_head) * V;
+        const unsigned token = part / (unsigned)a.chunks;
+        const int head0 = (int)(part - token * (unsigned)a.chunks) * a.chunk;
+        if (token >= a.tokens) return;
+        long long at[3];
+        if (a.positions) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                T &first_of = INTERLEAVED ? (2 * e < V ? va.v[(2 * e) % V] : vb.v[(2 * e) % V]) : va.v[e];
-                T &second_of = INTERLEAVED ? (2 * e + 1 < V ? va.v[(2 * e + 1) % V] : vb.v[(2 * e + 1) % V]) : vb.v[e];
-                const float p = to_float<T>(first_of), q = to_float<T>(second_of);
-                first_of = from_float<T>(p * cs[e].x - q * cs[e].y);
-                second_of = from_float<T>(p * cs[e].y + q * cs[e].x);
-            }
-            *reinterpret_cast<Raw *>(dst + at_a) = va.raw;
-            *reinterpret_cast<Raw *>(dst + at_b) = vb.raw;
-        }
-        if (!copies) continue;
-        for (int i = threadIdx.x; i < count * a.heads * rest; i += ROPE_THREADS) {
-            const int k = i / (a.heads * rest), r = i - k * a.heads * rest;
-            const int at = r / rest * a.head_dim + 2 * a.pairs + r % rest * V;
-            *reinterpret_cast<Raw *>(y + (size_t)(first + k) * a.yp + at) = *reinterpret_cast<const Raw *>(x + (size_t)(first + k) * a.xp + at);
-        }
-        if ((tail0 & 7) == 0) {
-            for (int i = threadIdx.x; i < count * tail; i += ROPE_THREADS) {
-                const int k = i / tail, at = tail0 + (i - k * tail) * 8;
-                const T *src = x + (size_t)(first + k) * a.xp + at;
-                T *dst = y + (size_t)(first + k) * a.yp + at;
-#pragma unroll
-                for (int b = 0; b < (int)sizeof(T) / 2; ++b) {                    // eight channels: one vector of bf16, two of f32
-                    constexpr int N = 16 / sizeof(T);
-                    union { uint4 raw; T v[N]; } v;
-                    v.raw = reinterpret_cast<const uint4 *>(src)[b];
-#pragma unroll
-                    for (int e = 0; e < N; ++e)
-                        if (at + b * N + e >= a.c) v.v[e] = from_float<T>(0.f);   // padding channels stay zero
-                    reinterpret_cast<uint4 *>(dst)[b] = v.raw;
-                }
-            }
+            for (int i = 0; i < 3; ++i) at[i] = a.positions[(size_t)token * 3 + i];
         } else {
-            for (int i = threadIdx.x; i < count * (a.c8 - tail0); i += ROPE_THREADS) {
-                const int k = i / (a.c8 - tail0), at = tail0 + i % (a.c8 - tail0);
-                y[(size_t)(first + k) * a.yp + at] = at < a.c ? x[(size_t)(first + k) * a.xp + at] : from_float<T>(0.f);
+            const unsigned row = token / (unsigned)a.w, image = row / (unsigned)a.h;
+            at[0] = (long long)(image % (unsigned)a.frames) + a.origin[0];
+            at[1] = (long long)(row - image * (unsigned)a.h) + a.origin[1];
+            at[2] = (long long)(token - row * (unsigned)a.w) + a.origin[2];
+        }
+        float cs[V], sn[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const int s = axis[j + e];
+            const uint64_t where = (uint64_t)(s == 0 ? at[0] : s == 1 ? at[1] : at[2]);
+            const int turns = (int)(where * turn[j + e] >> 32);                   // signed: from -1/2 to 1/2 of a turn, in units of 2^-32
+            // bf16: the hardware's sine, off by 2^-21.4 at most on one turn, where half a step of the output is 2^-9 or more of it
+            if (sizeof(T) == 2) __sincosf((float)turns * (6.283185307179586f * 0x1p-32f), &sn[e], &cs[e]);
+            else sincospif((float)turns * 0x1p-31f, &sn[e], &cs[e]);
+        }
+        const int at_a = INTERLEAVED ? 2 * j : j, apart = INTERLEAVED ? V : a.pairs, count = min(a.chunk, a.heads - head0);
+        const T *src = x + (size_t)token * a.xp + head0 * a.head_dim + at_a;
+        T *dst = y + (size_t)token * a.yp + head0 * a.head_dim + at_a;
+        for (int h0 = 0; h0 < count; h0 += AT_ONCE, src += AT_ONCE * a.head_dim, dst += AT_ONCE * a.head_dim) {
+            Vec va[AT_ONCE], vb[AT_ONCE];
+#pragma unroll
+            for (int h = 0; h < AT_ONCE; ++h)
+                if (h0 + h < count) {
+                    va[h].raw = *reinterpret_cast<const Raw *>(src + h * a.head_dim);
+                    vb[h].raw = *reinterpret_cast<const Raw *>(src + h * a.head_dim + apart);
+                }
+#pragma unroll
+            for (int h = 0; h < AT_ONCE; ++h)
+                if (h0 + h < count) {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        T &first = INTERLEAVED ? (2 * e < V ? va[h].v[(2 * e) % V] : vb[h].v[(2 * e) % V]) : va[h].v[e];
+                        T &second = INTERLEAVED ? (2 * e + 1 < V ? va[h].v[(2 * e + 1) % V] : vb[h].v[(2 * e + 1) % V]) : vb[h].v[e];
+                        const float p = to_float<T>(first), q = to_float<T>(second);
+                        first = from_float<T>(p * cs[e] - q * sn[e]);
+                        second = from_float<T>(p * sn[e] + q * cs[e]);
+                    }
+                    *reinterpret_cast<Raw *>(dst + h * a.head_dim) = va[h].raw;
+                    *reinterpret_cast<Raw *>(dst + h * a.head_dim + apart) = vb[h].raw;
+                }
+        }
+        return;
+    }
+    // What passes: of each head the channels behind its pairs, by V, and the channels behind the heads, by eights (by one where they start off a vector).
+    const int rest = (a.head_dim - 2 * a.pairs) / V, tail0 = a.heads * a.head_dim, unit = tail0 & 7 ? 1 : 8, tail = (a.c8 - tail0) / unit;
+    const unsigned per_token = (unsigned)(a.heads * rest + tail);
+    const unsigned long long total = (unsigned long long)a.tokens * per_token, step = (unsigned long long)(gridDim.x - a.turners) * ROPE_THREADS;
+    for (unsigned long long i = (unsigned long long)(blockIdx.x - a.turners) * ROPE_THREADS + threadIdx.x; i < total; i += step) {
+        const unsigned token = (unsigned)(i / per_token);
+        const int r = (int)(i - (unsigned long long)token * per_token);
+        const T *src = x + (size_t)token * a.xp;
+        T *dst = y + (size_t)token * a.yp;
+        if (r < a.heads * rest) {
+            const int at = r / rest * a.head_dim + 2 * a.pairs + r % rest * V;
+            *reinterpret_cast<Raw *>(dst + at) = *reinterpret_cast<const Raw *>(src + at);
+        } else if (unit == 1) {
+            const int at = tail0 + r - a.heads * rest;
+            dst[at] = at < a.c ? src[at] : from_float<T>(0.f);
+        } else {
+            const int at = tail0 + (r - a.heads * rest) * 8;
+            constexpr int N = 16 / sizeof(T);
+#pragma unroll
+            for (int b = 0; b < 8 / N; ++b) {                                     // eight channels: one vector of bf16, two of f32
+                union { uint4 raw; T v[N]; } v;
+                v.raw = reinterpret_cast<const uint4 *>(src + at)[b];
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (at + b * N + e >= a.c) v.v[e] = from_float<T>(0.f);       // padding channels stay zero
+                reinterpret_cast<uint4 *>(dst + at)[b] = v.raw;
             }
         }
     }
 }
 
 template <typename T, int V>
-static cudaError_t start_rope(const RopeArgs &a, bool interleaved, int grid, cudaStream_t s)
+static cudaError_t start_rope(const RopeArgs &a, bool interleaved, unsigned grid, cudaStream_t s)
 {
     return interleaved ? launch_overlapped(rope_kernel<T, V, true>, grid, ROPE_THREADS, 0, s, a) : launch_overlapped(rope_kernel<T, V, false>, grid, ROPE_THREADS, 0, s, a);
 }
@@ -154,12 +168,13 @@ static int launch_rope(const dnb_rope_plan &p, const dnb_tensor *x, const int32_
     if (x->data == y->data && x->cpitch != y->cpitch) DNB_FAIL(DNB_EINVAL, "rope: in place with another cpitch");
     if (positions && (uintptr_t)positions % 4) DNB_FAIL(DNB_EINVAL, "rope: positions must be 4-byte aligned");
     if (!positions && x->n % d.frames) DNB_FAIL(DNB_EINVAL, "rope: %d images are no whole number of clips of %d frames", x->n, d.frames);
-    if ((long long)x->n * x->h >= 1LL << 31) DNB_FAIL(DNB_EUNSUPPORTED, "rope: %d x %d rows", x->n, x->h);
+    const long long tokens = (long long)x->n * x->h * x->w;
+    if ((long long)x->n * x->h >= 1LL << 31 || tokens >= 1LL << 31) DNB_FAIL(DNB_EUNSUPPORTED, "rope: 2^31 tokens or more");
     RopeArgs a;
     memcpy(a.turn, p.turn, sizeof(a.turn));
     memcpy(a.axis, p.axis, sizeof(a.axis));
     a.x = x->data; a.y = y->data; a.positions = positions;
-    a.tokens = (long long)x->n * x->h * x->w;
+    a.tokens = (unsigned)tokens;
     a.xp = x->cpitch; a.yp = y->cpitch;
     a.c = x->c; a.c8 = round_up(x->c, 8);
     a.h = x->h; a.w = x->w; a.frames = d.frames;
@@ -168,13 +183,18 @@ static int launch_rope(const dnb_rope_plan &p, const dnb_tensor *x, const int32_
     // the widest vector that the pairs and the heads are whole numbers of
     int v = x->dtype == DNB_BF16 ? 8 : 4;
     while (p.pairs % v || d.head_dim % v) v /= 2;
-    // Tokens of a tile: about two items a thread, so that a sine is there for two or more of them; as many as the table holds.
-    const int per_token = d.heads * (p.pairs / v);
-    int tile = (2 * ROPE_THREADS + per_token - 1) / per_token;
-    if (tile > ROPE_TABLE / p.pairs) tile = ROPE_TABLE / p.pairs;
-    a.tile = tile;
-    const long long tiles = (a.tokens + tile - 1) / tile, cap = (long long)sm_count() * 8;
-    const int grid = (int)(tiles < cap ? tiles : cap);
+    // Heads of a thread: eight, so that its sines cost it little; fewer while there are too few threads to fill the GPU.
+    const int per_head = p.pairs / v;
+    a.chunk = d.heads < 8 ? d.heads : 8;
+    while (a.chunk > 1 && tokens * per_head * ((d.heads + a.chunk - 1) / a.chunk) < (long long)sm_count() * 1024) a.chunk = (a.chunk + 1) / 2;
+    a.chunks = (d.heads + a.chunk - 1) / a.chunk;
+    if (tokens * a.chunks >= 1LL << 31) { a.chunk = d.heads; a.chunks = 1; }
+    const unsigned long long turners = ((unsigned long long)tokens * a.chunks * per_head + ROPE_THREADS - 1) / ROPE_THREADS;
+    const long long passing = x->data == y->data ? 0 : d.heads * (long long)((d.head_dim - 2 * p.pairs) / v) + (a.c8 - d.heads * d.head_dim + 7) / 8;
+    const long long copiers = (tokens * passing + 4 * ROPE_THREADS - 1) / (4 * ROPE_THREADS), most = (long long)sm_count() * 16;
+    if (turners + most >= 1ULL << 31) DNB_FAIL(DNB_EUNSUPPORTED, "rope: %lld tokens", tokens);
+    a.turners = (unsigned)turners;
+    const unsigned grid = a.turners + (unsigned)(copiers < most ? copiers : most);
     cudaError_t e;
     if (x->dtype == DNB_BF16) {
         using T = __nv_bfloat16;
