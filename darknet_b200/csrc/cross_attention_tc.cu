@@ -15,6 +15,7 @@
 // Few rows: the keys of one pair of tiles are split over the CTAs of a cluster, which join their sums through distributed shared memory: no
 // workspace, one launch, the same order of additions every time.
 #include <atomic>
+#include <type_traits>
 
 #include "attention.cuh"
 
@@ -29,10 +30,11 @@ namespace {
 constexpr int THREADS = 320;                      // two warpgroups of softmax, a warp for the loads, one for the products
 constexpr int MAX_STAGES = 12;
 constexpr uint32_t BOX_BYTES = 128 * 128;         // 64 channels of 128 rows
+constexpr int FMA_EVERY = 4;                      // every how many-th pair of exponentials goes to the FMA pipe
 constexpr float MOVE = 8.f;                       // how far (log2) scores may outgrow the running maximum
 
 struct Shared {
-    uint64_t q_full, full[MAX_STAGES], empty[MAX_STAGES], s_full[2], p_full[2], o_full[2];
+    uint64_t q_full, full[MAX_STAGES], empty[MAX_STAGES], s_full[2], s_read[2], p_full[2], o_full[2];
     uint32_t tmem_base;
     int abort_flag;
     float top[256], sum[256];                     // of the rows, for the join
@@ -67,6 +69,40 @@ __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t *r)
           "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// Waits for the loads so far; the values pass through it, so that nothing that uses them is moved in front of it.
+__device__ __forceinline__ void tmem_ld_wait32(uint32_t *r)
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                   "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                   "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// 2^x of two x <= 120 by the FMA pipe, beside the exponentials of the other pipe: x = n + f with n its nearest whole number (left in the low bits by
+// an addition of 1.5 * 2^23), 2^f by a polynomial of degree 4 fitted to the smallest largest relative error on [-1/2, 1/2] (2.6e-6; the weights are
+// rounded to 2^-8 next), n added to the exponent.  x below -126 counts as -126.
+__device__ __forceinline__ void exp2_by_fma(uint64_t x2, float &a, float &b)
+{
+    const uint64_t magic = pack2(12582912.f, 12582912.f), back = pack2(-12582912.f, -12582912.f), minus = pack2(-1.f, -1.f);
+    float x, y, nx, ny, px, py;
+    unpack2(x2, x, y);
+    x2 = pack2(fmaxf(x, -126.f), fmaxf(y, -126.f));
+    const uint64_t n = add2(x2, magic), f = fma2(add2(n, back), minus, x2);
+    uint64_t p = fma2(f, pack2(0x1.3997d2p-7f, 0x1.3997d2p-7f), pack2(0x1.ca1440p-5f, 0x1.ca1440p-5f));
+    p = fma2(p, f, pack2(0x1.ec06dap-3f, 0x1.ec06dap-3f));
+    p = fma2(p, f, pack2(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
+    p = fma2(p, f, pack2(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
+    unpack2(n, nx, ny);
+    unpack2(p, px, py);
+    a = __uint_as_float((__float_as_uint(nx) << 23) + __float_as_uint(px));
+    b = __uint_as_float((__float_as_uint(ny) << 23) + __float_as_uint(py));
+}
 
 // V as it lies in shared memory: rows of 64 channels (128 bytes, swizzled), a key each: N is contiguous.  Blocks of 64 channels are a box
 // apart, groups of eight keys 1024 bytes.
@@ -79,13 +115,21 @@ __device__ __forceinline__ uint64_t desc_values(uint32_t addr)
     d |= (uint64_t)2 << 61;
     return d;
 }
+template <bool ADD>
 __device__ __forceinline__ void umma_from_tmem(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate)
 {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+    if (ADD)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.eq.b32 p, 0, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+            ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc) : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+            ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
 }
+
 // DP: channels of a head as they lie in shared memory, 64 or 128 (TMA fills what the head does not have with zeros).
 template <int DP> struct Cfg {
     static constexpr int BOXES = DP / 64;
@@ -93,6 +137,10 @@ template <int DP> struct Cfg {
     static constexpr int STAGES = DP == 128 ? 5 : 12;
     static constexpr uint32_t WORK = 2 * TILE_BYTES + STAGES * TILE_BYTES;
     static constexpr int PITCH = DP + 4;          // of a row of sums, for the join
+    // TMEM: the scores of both tiles, their outputs and, where there is room, weights of their own.  Then the next tile's scores are made while the
+    // weights of this one are; heads of more than 64 channels have the weights in the scores' place, and the next scores wait for their product.
+    static constexpr bool OWN_P = DP == 64;
+    static constexpr uint32_t O_AT = 256, P_AT = OWN_P ? 256 + 2 * DP : 0, P_STEP = OWN_P ? 64 : 128;
     static_assert(256 * PITCH * 4 <= WORK && STAGES <= MAX_STAGES, "the rows' sums fit where the operands were");
     static_assert(WORK + sizeof(Shared) <= 232448, "");
 };
@@ -127,6 +175,7 @@ attention_tc_kernel(const __grid_constant__ TcAttnArgs t)
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&sh->s_full[i]), 1);
+            mbar_init(smem_u32(&sh->s_read[i]), 4);
             mbar_init(smem_u32(&sh->p_full[i]), 4);
             mbar_init(smem_u32(&sh->o_full[i]), 1);
         }
@@ -145,7 +194,8 @@ attention_tc_kernel(const __grid_constant__ TcAttnArgs t)
     launch_dependents_if_small();
     const uint32_t tmem = sh->tmem_base;
     auto s_cols = [&](int s) { return tmem + 128 * s; };
-    auto o_cols = [&](int s) { return tmem + 256 + DP * s; };
+    auto o_cols = [&](int s) { return tmem + C::O_AT + DP * s; };
+    auto p_cols = [&](int s) { return tmem + C::P_AT + C::P_STEP * s; };
 
     int keys = a.lk;
     if (a.lengths) keys = min(max(a.lengths[image], 0), a.lk);
@@ -183,53 +233,103 @@ attention_tc_kernel(const __grid_constant__ TcAttnArgs t)
         const int qk_steps = (a.d + 15) >> 4;
         const uint32_t idesc_qk = mma_idesc<MMA_BF16>(128, 128) | (t.negate ? 1u << 13 : 0u);                     // bit 13: A, negated
         const uint32_t idesc_pv = mma_idesc<MMA_BF16>(128, (uint32_t)(qk_steps * 16)) | 1u << 16;                 // bit 16: B's rows are contiguous along N
-        auto scores = [&](int s, uint32_t k_smem) {
+        const uint64_t dq = make_smem_desc(q_smem, 128), dk = make_smem_desc(ring, 128), dv = desc_values(ring);
+        constexpr uint64_t SLOT = C::TILE_BYTES >> 4;
+        // Descriptors are a base and constants, products are unrolled: with their addresses made one by one the issue of a product took 55 clocks, as long
+        // as the product.
+        auto scores = [&](int s, int slot) {
             if (elect_one()) {
-                for (int i = 0; i < qk_steps; ++i) {
-                    const uint32_t off = (i >> 2) * BOX_BYTES + (i & 3) * 32;
-                    umma<MMA_BF16>(s_cols(s), make_smem_desc(q_smem + s * C::TILE_BYTES + off, 128), make_smem_desc(k_smem + off, 128), idesc_qk, i > 0);
+                const uint64_t q = dq + s * SLOT, k = dk + slot * SLOT;
+                if (qk_steps == DP / 16) {
+                    umma<MMA_BF16>(s_cols(s), q, k, idesc_qk, 0u);
+#pragma unroll
+                    for (int i = 1; i < DP / 16; ++i) {
+                        const uint64_t off = ((i >> 2) * BOX_BYTES + (i & 3) * 32) >> 4;
+                        umma<MMA_BF16>(s_cols(s), q + off, k + off, idesc_qk, 1u);
+                    }
+                } else {
+                    for (int i = 0; i < qk_steps; ++i) {
+                        const uint64_t off = ((i >> 2) * BOX_BYTES + (i & 3) * 32) >> 4;
+                        umma<MMA_BF16>(s_cols(s), q + off, k + off, idesc_qk, i > 0);
+                    }
                 }
                 umma_commit(smem_u32(&sh->s_full[s]));
             }
         };
+        auto output = [&](int s, int slot, uint32_t add, bool done) {
+            if (elect_one()) {
+                const uint64_t v = dv + slot * SLOT;
+                umma_from_tmem<false>(o_cols(s), p_cols(s), v, idesc_pv, add);
+#pragma unroll
+                for (int i = 1; i < 8; ++i) umma_from_tmem<true>(o_cols(s), p_cols(s) + 8 * i, v + i * (2048 >> 4), idesc_pv, 1u);
+                if (done) umma_commit(smem_u32(&sh->o_full[s]));
+            }
+        };
+        auto release = [&](int slot) {
+            if (elect_one()) umma_commit(smem_u32(&sh->empty[slot]));
+        };
+        auto landed = [&](int slot, uint32_t phase, int code) { return mbar_wait_warp(smem_u32(&sh->full[slot]), phase, abort_flag, a.status, code, a.wait_limit); };
         // slot 2j of the ring is K's tile j, slot 2j + 1 V's
         int stage = 0;
         uint32_t phase = 0;
         auto next = [&]() { if (++stage == C::STAGES) { stage = 0; phase ^= 1; } };
-        if (ok) ok = mbar_wait_warp(smem_u32(&sh->full[0]), 0, abort_flag, a.status, AT_KEYS, a.wait_limit);
+        ok = ok && landed(0, 0, AT_KEYS);
         if (ok) {
-            for (int s = 0; s < sides; ++s) scores(s, ring);
-            if (elect_one()) umma_commit(smem_u32(&sh->empty[0]));
+            scores(0, 0);
+            if (sides == 2) scores(1, 0);
+            release(0);
             next();
         }
         for (int j = 0; ok && j < tiles; ++j) {
-            const int v_stage = stage;
+            const int v_slot = stage;
             const uint32_t v_phase = phase;
             next();
-            const int k_stage = stage;
+            const int k_slot = stage;
             const uint32_t k_phase = phase;
             const bool more = j + 1 < tiles;
             if (more) next();
-            if (!mbar_wait_warp(smem_u32(&sh->full[v_stage]), v_phase, abort_flag, a.status, AT_VALUES, a.wait_limit)) { ok = false; break; }
-            for (int s = 0; s < sides; ++s) {
-                if (!mbar_wait_warp(smem_u32(&sh->p_full[s]), j & 1, abort_flag, a.status, AT_WEIGHTS, a.wait_limit)) { ok = false; break; }
-                tc_fence_after();
-                if (elect_one()) {
-                    const uint32_t v_smem = ring + v_stage * C::TILE_BYTES;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) umma_from_tmem(o_cols(s), s_cols(s) + 8 * i, desc_values(v_smem + i * 2048), idesc_pv, j > 0 || i > 0);
-                    if (s == sides - 1) umma_commit(smem_u32(&sh->empty[v_stage]));
-                    if (!more) umma_commit(smem_u32(&sh->o_full[s]));
-                }
+            if constexpr (C::OWN_P) {
                 if (more) {
-                    if (s == 0 && !mbar_wait_warp(smem_u32(&sh->full[k_stage]), k_phase, abort_flag, a.status, AT_KEYS, a.wait_limit)) { ok = false; break; }
-                    scores(s, ring + k_stage * C::TILE_BYTES);
-                    if (s == sides - 1 && elect_one()) umma_commit(smem_u32(&sh->empty[k_stage]));
+                    if (!(ok = landed(k_slot, k_phase, AT_KEYS))) break;
+#pragma unroll
+                    for (int s = 0; s < 2; ++s)
+                        if (s < sides && ok) {
+                            ok = mbar_wait_warp(smem_u32(&sh->s_read[s]), j & 1, abort_flag, a.status, AT_SCORES, a.wait_limit);
+                            tc_fence_after();
+                            if (ok) scores(s, k_slot);
+                        }
+                    if (!ok) break;
+                    release(k_slot);
                 }
+                if (!(ok = landed(v_slot, v_phase, AT_VALUES))) break;
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+                    if (s < sides && ok) {
+                        ok = mbar_wait_warp(smem_u32(&sh->p_full[s]), j & 1, abort_flag, a.status, AT_WEIGHTS, a.wait_limit);
+                        tc_fence_after();
+                        if (ok) output(s, v_slot, j > 0, true);
+                    }
+                if (!ok) break;
+                release(v_slot);
+            } else {
+                if (!(ok = landed(v_slot, v_phase, AT_VALUES))) break;
+                if (more && !(ok = landed(k_slot, k_phase, AT_KEYS))) break;
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+                    if (s < sides && ok) {
+                        ok = mbar_wait_warp(smem_u32(&sh->p_full[s]), j & 1, abort_flag, a.status, AT_WEIGHTS, a.wait_limit);
+                        tc_fence_after();
+                        if (ok) {
+                            output(s, v_slot, j > 0, !more);
+                            if (more) scores(s, k_slot);
+                        }
+                    }
+                if (!ok) break;
+                release(v_slot);
+                if (more) release(k_slot);
             }
         }
     }
-
     __syncwarp();
 
     // ---------------------------------------------------------------- softmax: a row a thread
@@ -273,22 +373,35 @@ attention_tc_kernel(const __grid_constant__ TcAttnArgs t)
             if (!mbar_wait(smem_u32(&sh->s_full[s]), j & 1, abort_flag, a.status, AT_SCORES, 0, a.wait_limit)) { ok = false; break; }
             tc_fence_after();
             uint32_t v[128];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_ld32(s_cols(s) + lanes + 32 * c, v + 32 * c);
-            tmem_ld_wait();
-            if (MASK || left < 128) {
-#pragma unroll
-                for (int c = 0; c < 128; ++c)
-                    if (!(bits[c >> 5] >> (c & 31) & 1)) v[c] = 0xff800000u;
-            }
             float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            tmem_ld32(s_cols(s) + lanes, v);
 #pragma unroll
-            for (int c = 0; c < 128; ++c) most[c & 3] = fmaxf(most[c & 3], __uint_as_float(v[c]));
-            const float grown = fmaxf(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])), top);
-            if (__any_sync(0xffffffffu, (grown - top) * scale > MOVE)) {
+            for (int c = 0; c < 128; c += 32) {
+                tmem_ld_wait32(v + c);
+                if (c + 32 < 128) tmem_ld32(s_cols(s) + lanes + c + 32, v + c + 32);      // travels while this quarter's largest is looked for
+                else if (C::OWN_P) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&sh->s_read[s]));
+                }
+                if (MASK || left < 128) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        if (!(bits[c >> 5] >> e & 1)) v[c + e] = 0xff800000u;
+                }
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) most[e / 2 & 3] = max3_nan(__uint_as_float(v[c + e]), __uint_as_float(v[c + e + 1]), most[e / 2 & 3]);
+            }
+            const float grown = max3_nan(max3_nan(most[0], most[1], most[2]), most[3], top);          // a NaN stays
+            // The tile before has to be out of O (its corrections) and, with a place of its own, of P.
+            if (C::OWN_P && j > 0) {
+                if (!mbar_wait(smem_u32(&sh->o_full[s]), (j - 1) & 1, abort_flag, a.status, AT_OUTPUT, 0, a.wait_limit)) { ok = false; break; }
+                tc_fence_after();
+            }
+            if (__any_sync(0xffffffffu, !((grown - top) * scale <= MOVE) && grown != -INFINITY)) {
                 const float shrink = grown == top ? 1.f : ex2((top - grown) * scale);
                 if (j > 0) {
-                    // every product of the tile before has retired: the scores' barrier came after them
+                    // (without a place of its own for P every product of the tile before has retired: the scores' barrier came after them)
 #pragma unroll 1
                     for (int c = 0; c < DP; c += 16) {
                         uint32_t o[16];
@@ -305,20 +418,30 @@ attention_tc_kernel(const __grid_constant__ TcAttnArgs t)
             const float base = top == -INFINITY ? 0.f : top * scale;
             const uint64_t scale2 = pack2(scale, scale), base2 = pack2(-base, -base);
             uint64_t sums[2] = {0, 0};
+            // A share of the exponentials by the other pipe; where something is hidden, or no number, all by the one that knows infinities.
+            const bool split = !MASK && left >= 128 && __all_sync(0xffffffffu, !valid || fabsf(top) < INFINITY);
+            auto weights = [&](auto by_fma) {
 #pragma unroll
-            for (int c = 0; c < 128; c += 32) {
-                uint32_t p[16];
+                for (int c = 0; c < 128; c += 32) {
+                    uint32_t p[16];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    float x, y;
-                    unpack2(fma2(pack2(__uint_as_float(v[c + 2 * e]), __uint_as_float(v[c + 2 * e + 1])), scale2, base2), x, y);
-                    x = ex2(x);
-                    y = ex2(y);
-                    sums[e & 1] = add2(sums[e & 1], pack2(x, y));
-                    p[e] = pack_bf16(x, y);
+                    for (int e = 0; e < 16; ++e) {
+                        const uint64_t x2 = fma2(pack2(__uint_as_float(v[c + 2 * e]), __uint_as_float(v[c + 2 * e + 1])), scale2, base2);
+                        float x, y;
+                        if (decltype(by_fma)::value && e % FMA_EVERY == FMA_EVERY - 1) exp2_by_fma(x2, x, y);
+                        else {
+                            unpack2(x2, x, y);
+                            x = ex2(x);
+                            y = ex2(y);
+                        }
+                        sums[e & 1] = add2(sums[e & 1], pack2(x, y));
+                        p[e] = pack_bf16(x, y);
+                    }
+                    tmem_st16(p_cols(s) + lanes + c / 2, p);
                 }
-                tmem_st16(s_cols(s) + lanes + c / 2, p);
-            }
+            };
+            if (split) weights(std::true_type{});
+            else weights(std::false_type{});
             float x0, x1, x2, x3;
             unpack2(sums[0], x0, x1);
             unpack2(sums[1], x2, x3);
@@ -345,7 +468,7 @@ attention_tc_kernel(const __grid_constant__ TcAttnArgs t)
             if (lane == 0) mbar_arrive(smem_u32(&sh->p_full[s]));
         }
         if (ok && tiles > 0) {
-            ok = mbar_wait(smem_u32(&sh->o_full[s]), 0, abort_flag, a.status, AT_OUTPUT, 0, a.wait_limit);
+            ok = mbar_wait(smem_u32(&sh->o_full[s]), C::OWN_P ? (tiles - 1) & 1 : 0, abort_flag, a.status, AT_OUTPUT, 0, a.wait_limit);
             tc_fence_after();
         }
     }
