@@ -25,7 +25,7 @@ struct AttnArgs {
     const uint8_t *mask;                    // or null
     long long mask_image, mask_query;       // its strides, bytes
     int *status;
-    long long wait_limit;
+    int polls;                              // bound of every device-side wait
     int debug;
 };
 

@@ -165,7 +165,10 @@ extern "C" int dnb_attention_forward(dnb_attention_plan *p, const dnb_tensor *q,
         a.lengths = mask->lengths;
         a.mask = mask->mask; a.mask_image = mask->image_stride; a.mask_query = a.lq > 1 ? mask->query_stride : 0;   // one query: one mask for all of them
     }
-    a.status = p->status; a.wait_limit = p->wait_limit; a.debug = p->debug;
+    a.status = p->status; a.debug = p->debug;
+    // a poll of a barrier that does not come takes about 2900 clocks: the hardware suspends the thread meanwhile
+    const long long polls = (p->wait_limit ? p->wait_limit : WAIT_LIMIT_CYCLES) / 2048 + 1;
+    a.polls = polls > 0x7fffffff ? 0x7fffffff : (int)polls;
     if (p->device < 0) DNB_FAIL(DNB_ECUDA, "attention: the plan was made without a CUDA device");
     DNB_TRY(check_current_device(p->device, "attention"));
     if (attention_rows_covers(a, q->dtype)) {

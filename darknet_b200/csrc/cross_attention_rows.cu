@@ -95,7 +95,7 @@ attention_rows_kernel(const __grid_constant__ RowsArgs t)
         uint32_t phase = 0;
         for (int i = 0; i < 2 * tiles; ++i) {
             const uint32_t full = smem_u32(&sh->full[stage]);
-            if (!mbar_wait_warp(smem_u32(&sh->empty[stage]), phase ^ 1, abort_flag, a.status, AT_SLOT, a.wait_limit)) break;
+            if (!mbar_wait_known(smem_u32(&sh->empty[stage]), phase ^ 1, abort_flag, a.status, AT_SLOT, a.polls)) break;
             if (elect_one() && !(a.debug & 32 && i == 1)) {
                 mbar_expect_tx(full, C::TILE);
                 for (int b = 0; b < C::BOXES; ++b)
@@ -108,7 +108,6 @@ attention_rows_kernel(const __grid_constant__ RowsArgs t)
 
     const int g = lane >> 2, c2 = (lane & 3) * 2;                       // this lane's rows g and g + 8 of a product, columns c2 and c2 + 1
     float o[DP / 8][4] = {}, top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
-    bool ok = true;
     if (warp < R_WARPS && tiles > 0) {
         uint32_t q[DP / 16][4];
 #pragma unroll
@@ -135,7 +134,7 @@ attention_rows_kernel(const __grid_constant__ RowsArgs t)
                     const int key = (i >> 1) * 8 + c2 + (i & 1);
                     in[e][i] = key < left && (!a.mask || mask[e][key0 + key]);
                 }
-            if (!mbar_wait(smem_u32(&sh->full[stage]), phase, abort_flag, a.status, AT_KEYS, 0, a.wait_limit)) { ok = false; break; }
+            mbar_wait_tight(smem_u32(&sh->full[stage]), phase, abort_flag, a.status, AT_KEYS, a.polls);
             float s[2][4] = {};
             {
                 const int key = warp * 16 + (m >> 1) * 8 + mr;
@@ -189,7 +188,7 @@ attention_rows_kernel(const __grid_constant__ RowsArgs t)
                     p[i * 2 + e] = pack_bf16(x, z);
                 }
             }
-            if (!mbar_wait(smem_u32(&sh->full[stage]), phase, abort_flag, a.status, AT_VALUES, 0, a.wait_limit)) { ok = false; break; }
+            mbar_wait_tight(smem_u32(&sh->full[stage]), phase, abort_flag, a.status, AT_VALUES, a.polls);
             const uint32_t v_tile = stage * C::TILE;
             if ((left < 16 && keys < a.lk) || (a.mask && a.mask_query == 0)) {
                 // values that no weight reaches may be anything: zeros in their place, this warp's keys by this warp
@@ -277,7 +276,6 @@ attention_rows_kernel(const __grid_constant__ RowsArgs t)
         const long long begin = clock64();
         while (clock64() - begin < 4000000LL) { }
     }
-    (void)ok;
 }
 
 typedef void (*RowsKernel)(RowsArgs);
@@ -293,7 +291,6 @@ int launch_attention_rows(const AttnArgs &a, cudaStream_t stream)
 {
     RowsArgs t;
     t.a = a;
-    if (!t.a.wait_limit) t.a.wait_limit = WAIT_LIMIT_CYCLES;
     t.scale_log2 = a.scale * 1.4426950408889634f;
     auto map = [&](CUtensorMap *m, const void *data, int pitch) {
         const uint64_t dims[4] = {(uint64_t)a.d, (uint64_t)a.kv_heads, (uint64_t)a.lk, (uint64_t)a.kn};

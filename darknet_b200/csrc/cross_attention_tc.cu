@@ -3,9 +3,9 @@
 // A CTA holds two tiles of 128 query rows (a row: one query token of one head; the heads that share keys lie side by side, so that their keys
 // are loaded once) and walks over the keys in tiles of 128:
 //   S = Q K^T   tcgen05.mma, both operands in shared memory by TMA, S in TMEM (fp32)
-//   P = exp2(S * scale * log2 e - m)   a warpgroup a tile, a row a thread, out of TMEM and back into it as bf16
+//   P = exp2(S * scale * log2 e - m)   eight warps a tile, half a row a thread, out of TMEM and back into it as bf16
 //   O += P V    tcgen05.mma, P from TMEM, V from shared memory as it lies (channels innermost: a transposed operand), O in TMEM (fp32)
-// While one tile's warpgroup takes exponentials, the tensor cores multiply the other tile's: the two are never both idle.
+// While one tile's warps take exponentials, the tensor cores multiply the other tile's: the two are never both idle.
 //
 // The running maximum m moves only when a row's largest score has outgrown it by more than 2^8 (every weight is then at most 256 times what
 // the largest should be, far inside bf16's and fp32's range); until then O needs no correction.  The sum of the weights is kept in fp32 of the
@@ -15,7 +15,6 @@
 // Few rows: the keys of one pair of tiles are split over the CTAs of a cluster, which join their sums through distributed shared memory: no
 // workspace, one launch, the same order of additions every time.
 #include <atomic>
-#include <type_traits>
 
 #include "attention.cuh"
 
@@ -27,17 +26,18 @@ int conv_tc_max_smem();
 
 namespace {
 
-constexpr int THREADS = 320;                      // two warpgroups of softmax, a warp for the loads, one for the products
+constexpr int SOFT_WARPS = 16, LOAD_WARP = 16, MMA_WARP = 17, THREADS = 20 * 32;
+// Registers: 640 threads start with 96 each; the four warps that load and multiply give 32 back, the sixteen others take 8 more: 512 * 104 + 128 * 64 = 640 * 96.
+constexpr int SOFT_REGS = 104, OTHER_REGS = 64;
 constexpr int MAX_STAGES = 12;
 constexpr uint32_t BOX_BYTES = 128 * 128;         // 64 channels of 128 rows
-constexpr int FMA_EVERY = 4;                      // every how many-th pair of exponentials goes to the FMA pipe
 constexpr float MOVE = 8.f;                       // how far (log2) scores may outgrow the running maximum
 
 struct Shared {
-    uint64_t q_full, full[MAX_STAGES], empty[MAX_STAGES], s_full[2], s_read[2], p_full[2], o_full[2];
+    uint64_t q_full, full[MAX_STAGES], empty[MAX_STAGES], s_full[2], s_read[2], p_full[2], o_full[2], met[8];
     uint32_t tmem_base;
     int abort_flag;
-    float top[256], sum[256];                     // of the rows, for the join
+    float halves[][2][256];                       // the largest scores of the rows' halves, and their sums at the end
 };
 
 struct alignas(64) TcAttnArgs {
@@ -84,26 +84,6 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c)
     return r;
 }
 
-// 2^x of two x <= 120 by the FMA pipe, beside the exponentials of the other pipe: x = n + f with n its nearest whole number (left in the low bits by
-// an addition of 1.5 * 2^23), 2^f by a polynomial of degree 4 fitted to the smallest largest relative error on [-1/2, 1/2] (2.6e-6; the weights are
-// rounded to 2^-8 next), n added to the exponent.  x below -126 counts as -126.
-__device__ __forceinline__ void exp2_by_fma(uint64_t x2, float &a, float &b)
-{
-    const uint64_t magic = pack2(12582912.f, 12582912.f), back = pack2(-12582912.f, -12582912.f), minus = pack2(-1.f, -1.f);
-    float x, y, nx, ny, px, py;
-    unpack2(x2, x, y);
-    x2 = pack2(fmaxf(x, -126.f), fmaxf(y, -126.f));
-    const uint64_t n = add2(x2, magic), f = fma2(add2(n, back), minus, x2);
-    uint64_t p = fma2(f, pack2(0x1.3997d2p-7f, 0x1.3997d2p-7f), pack2(0x1.ca1440p-5f, 0x1.ca1440p-5f));
-    p = fma2(p, f, pack2(0x1.ec06dap-3f, 0x1.ec06dap-3f));
-    p = fma2(p, f, pack2(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
-    p = fma2(p, f, pack2(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
-    unpack2(n, nx, ny);
-    unpack2(p, px, py);
-    a = __uint_as_float((__float_as_uint(nx) << 23) + __float_as_uint(px));
-    b = __uint_as_float((__float_as_uint(ny) << 23) + __float_as_uint(py));
-}
-
 // V as it lies in shared memory: rows of 64 channels (128 bytes, swizzled), a key each: N is contiguous.  Blocks of 64 channels are a box
 // apart, groups of eight keys 1024 bytes.
 __device__ __forceinline__ uint64_t desc_values(uint32_t addr)
@@ -134,15 +114,18 @@ __device__ __forceinline__ void umma_from_tmem(uint32_t tmem_d, uint32_t tmem_a,
 template <int DP> struct Cfg {
     static constexpr int BOXES = DP / 64;
     static constexpr uint32_t TILE_BYTES = BOXES * BOX_BYTES;
-    static constexpr int STAGES = DP == 128 ? 5 : 12;
+    static constexpr int STAGES = DP == 128 ? 5 : 11;
     static constexpr uint32_t WORK = 2 * TILE_BYTES + STAGES * TILE_BYTES;
     static constexpr int PITCH = DP + 4;          // of a row of sums, for the join
     // TMEM: the scores of both tiles, their outputs and, where there is room, weights of their own.  Then the next tile's scores are made while the
     // weights of this one are; heads of more than 64 channels have the weights in the scores' place, and the next scores wait for their product.
     static constexpr bool OWN_P = DP == 64;
     static constexpr uint32_t O_AT = 256, P_AT = OWN_P ? 256 + 2 * DP : 0, P_STEP = OWN_P ? 64 : 128;
-    static_assert(256 * PITCH * 4 <= WORK && STAGES <= MAX_STAGES, "the rows' sums fit where the operands were");
-    static_assert(WORK + sizeof(Shared) <= 232448, "");
+    // The halves' largest scores: one set for each of two tiles of keys where the next scores may be there before this tile's have been compared.
+    static constexpr int SETS = OWN_P ? 2 : 1;
+    static constexpr uint32_t BYTES = WORK + sizeof(Shared) + SETS * 2048;
+    static_assert(258 * PITCH * 4 + 2048 <= WORK && STAGES <= MAX_STAGES, "the rows' sums fit where the operands were");
+    static_assert(BYTES <= 232448, "fits an SM");
 };
 
 template <int DP, bool MASK>
@@ -175,15 +158,16 @@ attention_tc_kernel(const __grid_constant__ TcAttnArgs t)
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&sh->s_full[i]), 1);
-            mbar_init(smem_u32(&sh->s_read[i]), 4);
-            mbar_init(smem_u32(&sh->p_full[i]), 4);
+            mbar_init(smem_u32(&sh->s_read[i]), 8);
+            mbar_init(smem_u32(&sh->p_full[i]), 8);
             mbar_init(smem_u32(&sh->o_full[i]), 1);
         }
+        for (int i = 0; i < 8; ++i) mbar_init(smem_u32(&sh->met[i]), 2);
         sh->abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == 9) {
+    if (warp == MMA_WARP) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh->tmem_base)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -202,7 +186,20 @@ attention_tc_kernel(const __grid_constant__ TcAttnArgs t)
     int t0, tiles;
     share_of_keys(keys, 128, rank, t.splits, t0, tiles);
 
-    if (warp == 8) {
+    auto cluster_done = [&]() {
+        __syncwarp();
+        cluster_sync_all();
+    };
+    auto finish = [&]() {
+        if (*abort_flag) {                                              // loads and products in flight end before their memory goes
+            const long long begin = clock64();
+            while (clock64() - begin < 4000000LL) { }
+        }
+        __syncthreads();
+    };
+    if (warp >= SOFT_WARPS) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
+    if (warp == LOAD_WARP) {
         // ---------------------------------------------------------------- loads
         if (tiles > 0) {
             const int kv_image = a.kn == 1 ? 0 : image;
@@ -218,7 +215,7 @@ attention_tc_kernel(const __grid_constant__ TcAttnArgs t)
             uint32_t phase = 0;
             for (int i = 0; i < 2 * tiles; ++i) {
                 const uint32_t full = smem_u32(&sh->full[stage]);
-                if (!mbar_wait_warp(smem_u32(&sh->empty[stage]), phase ^ 1, abort_flag, a.status, AT_SLOT, a.wait_limit)) break;
+                if (!mbar_wait_known(smem_u32(&sh->empty[stage]), phase ^ 1, abort_flag, a.status, AT_SLOT, a.polls)) break;
                 if (elect_one() && !(a.debug & 32 && i == 1)) {
                     mbar_expect_tx(full, C::TILE_BYTES);
                     for (int b = 0; b < C::BOXES; ++b)
@@ -227,9 +224,9 @@ attention_tc_kernel(const __grid_constant__ TcAttnArgs t)
                 if (++stage == C::STAGES) { stage = 0; phase ^= 1; }
             }
         }
-    } else if (warp == 9) {
+    } else if (warp == MMA_WARP) {
         // ---------------------------------------------------------------- products
-        bool ok = tiles > 0 && mbar_wait_warp(smem_u32(&sh->q_full), 0, abort_flag, a.status, AT_QUERIES, a.wait_limit);
+        bool ok = tiles > 0 && mbar_wait_known(smem_u32(&sh->q_full), 0, abort_flag, a.status, AT_QUERIES, a.polls);
         const int qk_steps = (a.d + 15) >> 4;
         const uint32_t idesc_qk = mma_idesc<MMA_BF16>(128, 128) | (t.negate ? 1u << 13 : 0u);                     // bit 13: A, negated
         const uint32_t idesc_pv = mma_idesc<MMA_BF16>(128, (uint32_t)(qk_steps * 16)) | 1u << 16;                 // bit 16: B's rows are contiguous along N
@@ -268,7 +265,7 @@ attention_tc_kernel(const __grid_constant__ TcAttnArgs t)
         auto release = [&](int slot) {
             if (elect_one()) umma_commit(smem_u32(&sh->empty[slot]));
         };
-        auto landed = [&](int slot, uint32_t phase, int code) { return mbar_wait_warp(smem_u32(&sh->full[slot]), phase, abort_flag, a.status, code, a.wait_limit); };
+        auto landed = [&](int slot, uint32_t phase, int code) { return mbar_wait_known(smem_u32(&sh->full[slot]), phase, abort_flag, a.status, code, a.polls); };
         // slot 2j of the ring is K's tile j, slot 2j + 1 V's
         int stage = 0;
         uint32_t phase = 0;
@@ -276,7 +273,12 @@ attention_tc_kernel(const __grid_constant__ TcAttnArgs t)
         ok = ok && landed(0, 0, AT_KEYS);
         if (ok) {
             scores(0, 0);
-            if (sides == 2) scores(1, 0);
+            if (sides == 2) {
+                // The tiles take turns: one looks for its largest scores while the other's exponentials go through.  Where each has its scores in time they
+                // stay as they start, and started together they keep both pipes waiting in turn (8 x 1444 x 5776 tokens, 8 heads of 64: 269 us, and 211 so).
+                if (C::OWN_P) ok = mbar_wait_known(smem_u32(&sh->s_read[0]), 0, abort_flag, a.status, AT_SCORES, a.polls);
+                if (ok) scores(1, 0);
+            }
             release(0);
             next();
         }
@@ -287,37 +289,39 @@ attention_tc_kernel(const __grid_constant__ TcAttnArgs t)
             const int k_slot = stage;
             const uint32_t k_phase = phase;
             const bool more = j + 1 < tiles;
-            if (more) next();
+            // operands first, while the weights are being made
+            ok = landed(v_slot, v_phase, AT_VALUES);
+            if (more) {
+                next();
+                ok = ok && landed(k_slot, k_phase, AT_KEYS);
+            }
+            if (!ok) break;
             if constexpr (C::OWN_P) {
                 if (more) {
-                    if (!(ok = landed(k_slot, k_phase, AT_KEYS))) break;
 #pragma unroll
                     for (int s = 0; s < 2; ++s)
                         if (s < sides && ok) {
-                            ok = mbar_wait_warp(smem_u32(&sh->s_read[s]), j & 1, abort_flag, a.status, AT_SCORES, a.wait_limit);
+                            ok = mbar_wait_known(smem_u32(&sh->s_read[s]), j & 1, abort_flag, a.status, AT_SCORES, a.polls);
                             tc_fence_after();
                             if (ok) scores(s, k_slot);
                         }
                     if (!ok) break;
                     release(k_slot);
                 }
-                if (!(ok = landed(v_slot, v_phase, AT_VALUES))) break;
 #pragma unroll
                 for (int s = 0; s < 2; ++s)
                     if (s < sides && ok) {
-                        ok = mbar_wait_warp(smem_u32(&sh->p_full[s]), j & 1, abort_flag, a.status, AT_WEIGHTS, a.wait_limit);
+                        ok = mbar_wait_known(smem_u32(&sh->p_full[s]), j & 1, abort_flag, a.status, AT_WEIGHTS, a.polls);
                         tc_fence_after();
                         if (ok) output(s, v_slot, j > 0, true);
                     }
                 if (!ok) break;
                 release(v_slot);
             } else {
-                if (!(ok = landed(v_slot, v_phase, AT_VALUES))) break;
-                if (more && !(ok = landed(k_slot, k_phase, AT_KEYS))) break;
 #pragma unroll
                 for (int s = 0; s < 2; ++s)
                     if (s < sides && ok) {
-                        ok = mbar_wait_warp(smem_u32(&sh->p_full[s]), j & 1, abort_flag, a.status, AT_WEIGHTS, a.wait_limit);
+                        ok = mbar_wait_known(smem_u32(&sh->p_full[s]), j & 1, abort_flag, a.status, AT_WEIGHTS, a.polls);
                         tc_fence_after();
                         if (ok) {
                             output(s, v_slot, j > 0, !more);
@@ -331,59 +335,70 @@ attention_tc_kernel(const __grid_constant__ TcAttnArgs t)
         }
     }
     __syncwarp();
+    __syncthreads();                                                    // as below, where the rows are joined
+    if (t.splits > 1) {
+        cluster_done();
+        cluster_done();
+    }
+    finish();
+    if (warp == MMA_WARP) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+    return;
+    }
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFT_REGS));
 
-    // ---------------------------------------------------------------- softmax: a row a thread
-    const int s = warp >> 2, row = tid & 127;
-    const bool mine = warp < 4 * sides && warp < 8;
+    // ---------------------------------------------------------------- softmax: half a row a thread
+    const int s = warp >> 3, half = warp >> 2 & 1, row = (warp & 3) * 32 + lane;
+    const bool mine = warp < 8 * sides;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;                  // this warp's lanes of TMEM
     const int r_token = token0 + s * t.q_tokens + row / a.group;
     const bool valid = mine && row < t.q_tokens * a.group && r_token < a.lq;
     float top = -INFINITY, sum = 0.f;
-    bool ok = true;
     if (mine) {
         const float scale = t.scale_log2;
+        const uint32_t met = smem_u32(&sh->met[s * 4 + (warp & 3)]);    // this warp and the one with the rows' other half
         const uint8_t *mask = nullptr;
         if (MASK) mask = a.mask + (long long)image * a.mask_image + (valid ? r_token : a.lq - 1) * a.mask_query;
         int stage = 1;
         uint32_t phase = 0;                                             // of V's slots
         for (int j = 0; j < tiles; ++j) {
-            const int key0 = (t0 + j) * 128, left = keys - key0;
-            uint32_t bits[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+            const int key0 = (t0 + j) * 128, left = keys - key0, col0 = half * 64;
+            uint32_t bits[2] = {0xffffffffu, 0xffffffffu};
             if (MASK) {
                 // The rows' masks, one row after another, 32 keys a load; rows of one query (heads that share keys) share the load.
                 const uint8_t *last = nullptr;
-                uint32_t now[4] = {0, 0, 0, 0};
+                uint32_t now[2] = {0, 0};
                 for (int i = 0; i < 32; ++i) {
                     const uint8_t *p = reinterpret_cast<const uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mask), i));
                     if (p != last) {
                         last = p;
-                        p += key0;
+                        p += key0 + col0;
 #pragma unroll
-                        for (int w = 0; w < 4; ++w) {
+                        for (int w = 0; w < 2; ++w) {
                             const int c = lane + 32 * w;
-                            now[w] = __ballot_sync(0xffffffffu, c < left && p[c] != 0);
+                            now[w] = __ballot_sync(0xffffffffu, col0 + c < left && p[c] != 0);
                         }
                     }
-                    if (lane == i) { bits[0] = now[0]; bits[1] = now[1]; bits[2] = now[2]; bits[3] = now[3]; }
+                    if (lane == i) { bits[0] = now[0]; bits[1] = now[1]; }
                 }
             } else if (left < 128) {
 #pragma unroll
-                for (int w = 0; w < 4; ++w) bits[w] = left >= 32 * w + 32 ? 0xffffffffu : left > 32 * w ? (1u << (left - 32 * w)) - 1u : 0u;
-            }
-            if (!mbar_wait(smem_u32(&sh->s_full[s]), j & 1, abort_flag, a.status, AT_SCORES, 0, a.wait_limit)) { ok = false; break; }
-            tc_fence_after();
-            uint32_t v[128];
-            float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            tmem_ld32(s_cols(s) + lanes, v);
-#pragma unroll
-            for (int c = 0; c < 128; c += 32) {
-                tmem_ld_wait32(v + c);
-                if (c + 32 < 128) tmem_ld32(s_cols(s) + lanes + c + 32, v + c + 32);      // travels while this quarter's largest is looked for
-                else if (C::OWN_P) {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(&sh->s_read[s]));
+                for (int w = 0; w < 2; ++w) {
+                    const int n = left - col0 - 32 * w;
+                    bits[w] = n >= 32 ? 0xffffffffu : n > 0 ? (1u << n) - 1u : 0u;
                 }
+            }
+            mbar_wait_tight(smem_u32(&sh->s_full[s]), j & 1, abort_flag, a.status, AT_SCORES, a.polls);
+            tc_fence_after();
+            uint32_t v[64];
+            float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            tmem_ld32(s_cols(s) + lanes + col0, v);
+#pragma unroll
+            for (int c = 0; c < 64; c += 32) {
+                tmem_ld_wait32(v + c);
+                if (c == 0) tmem_ld32(s_cols(s) + lanes + col0 + 32, v + 32);             // travels while the first ones' largest is looked for
                 if (MASK || left < 128) {
 #pragma unroll
                     for (int e = 0; e < 32; ++e)
@@ -392,18 +407,30 @@ attention_tc_kernel(const __grid_constant__ TcAttnArgs t)
 #pragma unroll
                 for (int e = 0; e < 32; e += 2) most[e / 2 & 3] = max3_nan(__uint_as_float(v[c + e]), __uint_as_float(v[c + e + 1]), most[e / 2 & 3]);
             }
-            const float grown = max3_nan(max3_nan(most[0], most[1], most[2]), most[3], top);          // a NaN stays
+            float grown = max3_nan(max3_nan(most[0], most[1], most[2]), most[3], top);    // a NaN stays
+            // The halves of a row meet.  After it both have read their scores: the weights may take their place.
+            sh->halves[j & (C::SETS - 1)][half][s * 128 + row] = grown;
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(met);
+                if (C::OWN_P) mbar_arrive(smem_u32(&sh->s_read[s]));
+            }
+            mbar_wait_tight(met, j & 1, abort_flag, a.status, AT_SCORES, a.polls);
+            tc_fence_after();
+            grown = max3_nan(grown, sh->halves[j & (C::SETS - 1)][half ^ 1][s * 128 + row], grown);
             // The tile before has to be out of O (its corrections) and, with a place of its own, of P.
             if (C::OWN_P && j > 0) {
-                if (!mbar_wait(smem_u32(&sh->o_full[s]), (j - 1) & 1, abort_flag, a.status, AT_OUTPUT, 0, a.wait_limit)) { ok = false; break; }
+                mbar_wait_tight(smem_u32(&sh->o_full[s]), (j - 1) & 1, abort_flag, a.status, AT_OUTPUT, a.polls);
                 tc_fence_after();
             }
             if (__any_sync(0xffffffffu, !((grown - top) * scale <= MOVE) && grown != -INFINITY)) {
                 const float shrink = grown == top ? 1.f : ex2((top - grown) * scale);
                 if (j > 0) {
-                    // (without a place of its own for P every product of the tile before has retired: the scores' barrier came after them)
+                    // each half its half of the channels (without a place of its own for P every product of the tile before has retired: the
+                    // scores' barrier came after them)
 #pragma unroll 1
-                    for (int c = 0; c < DP; c += 16) {
+                    for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 16) {
                         uint32_t o[16];
                         tmem_ld16(o_cols(s) + lanes + c, o);
                         tmem_ld_wait();
@@ -418,43 +445,32 @@ attention_tc_kernel(const __grid_constant__ TcAttnArgs t)
             const float base = top == -INFINITY ? 0.f : top * scale;
             const uint64_t scale2 = pack2(scale, scale), base2 = pack2(-base, -base);
             uint64_t sums[2] = {0, 0};
-            // A share of the exponentials by the other pipe; where something is hidden, or no number, all by the one that knows infinities.
-            const bool split = !MASK && left >= 128 && __all_sync(0xffffffffu, !valid || fabsf(top) < INFINITY);
-            auto weights = [&](auto by_fma) {
 #pragma unroll
-                for (int c = 0; c < 128; c += 32) {
-                    uint32_t p[16];
+            for (int c = 0; c < 64; c += 32) {
+                uint32_t p[16];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const uint64_t x2 = fma2(pack2(__uint_as_float(v[c + 2 * e]), __uint_as_float(v[c + 2 * e + 1])), scale2, base2);
-                        float x, y;
-                        if (decltype(by_fma)::value && e % FMA_EVERY == FMA_EVERY - 1) exp2_by_fma(x2, x, y);
-                        else {
-                            unpack2(x2, x, y);
-                            x = ex2(x);
-                            y = ex2(y);
-                        }
-                        sums[e & 1] = add2(sums[e & 1], pack2(x, y));
-                        p[e] = pack_bf16(x, y);
-                    }
-                    tmem_st16(p_cols(s) + lanes + c / 2, p);
+                for (int e = 0; e < 16; ++e) {
+                    float x, y;
+                    unpack2(fma2(pack2(__uint_as_float(v[c + 2 * e]), __uint_as_float(v[c + 2 * e + 1])), scale2, base2), x, y);
+                    x = ex2(x);
+                    y = ex2(y);
+                    sums[e & 1] = add2(sums[e & 1], pack2(x, y));
+                    p[e] = pack_bf16(x, y);
                 }
-            };
-            if (split) weights(std::true_type{});
-            else weights(std::false_type{});
-            float x0, x1, x2, x3;
-            unpack2(sums[0], x0, x1);
-            unpack2(sums[1], x2, x3);
-            sum += (x0 + x1) + (x2 + x3);
+                tmem_st16(p_cols(s) + lanes + (col0 + c) / 2, p);
+            }
+            float x0, x1;
+            unpack2(add2(sums[0], sums[1]), x0, x1);
+            sum += x0 + x1;
             // Values that no weight reaches may be anything, and zero times infinity is no number: zeros in their place.  (Both tiles write them.)
             if ((left < 128 && keys < a.lk) || (MASK && a.mask_query == 0)) {
-                if (!mbar_wait(smem_u32(&sh->full[stage]), phase, abort_flag, a.status, AT_VALUES, 0, a.wait_limit)) { ok = false; break; }
+                mbar_wait_tight(smem_u32(&sh->full[stage]), phase, abort_flag, a.status, AT_VALUES, a.polls);
                 bool hidden = row >= left;
                 if (MASK && a.mask_query == 0 && !hidden) hidden = mask[key0 + row] == 0;
                 if (hidden) {
                     const uint32_t at = 2 * C::TILE_BYTES + stage * C::TILE_BYTES + row * 128;
 #pragma unroll
-                    for (int b = 0; b < C::BOXES; ++b)
+                    for (int b = half; b < C::BOXES; b += 2)
 #pragma unroll
                         for (int e = 0; e < 8; ++e) *reinterpret_cast<uint4 *>(smem_raw + at + b * BOX_BYTES + e * 16) = make_uint4(0, 0, 0, 0);
                 }
@@ -467,19 +483,23 @@ attention_tc_kernel(const __grid_constant__ TcAttnArgs t)
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&sh->p_full[s]));
         }
-        if (ok && tiles > 0) {
-            ok = mbar_wait(smem_u32(&sh->o_full[s]), C::OWN_P ? (tiles - 1) & 1 : 0, abort_flag, a.status, AT_OUTPUT, 0, a.wait_limit);
+        if (tiles > 0) {
+            mbar_wait_tight(smem_u32(&sh->o_full[s]), C::OWN_P ? (tiles - 1) & 1 : 0, abort_flag, a.status, AT_OUTPUT, a.polls);
             tc_fence_after();
         }
+        sh->halves[0][half][s * 128 + row] = sum;                       // the other half has compared its last: its weights were waited for
     }
+    __syncthreads();                                                    // every product has read its operands, too
+    if (mine) sum = sh->halves[0][0][s * 128 + row] + sh->halves[0][1][s * 128 + row];
 
     const bool wide = a.d % 16 == 0 && a.yp % 16 == 0 && (uintptr_t)a.y % 32 == 0;   // whole 32-byte sectors
     __nv_bfloat16 *y = (__nv_bfloat16 *)a.y + ((size_t)image * a.lq + r_token) * a.yp + (kv_head * a.group + row % a.group) * a.d;
+    const int o0 = half * (DP / 2), o1 = min(o0 + DP / 2, a.d);         // this thread's channels
     if (t.splits == 1) {
-        if (mine && ok) {
+        if (mine) {
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll 1
-            for (int c = 0; c < a.d; c += 16) {
+            for (int c = o0; c < o1; c += 16) {
                 uint32_t o[16], p[8];
                 if (tiles > 0) {
                     tmem_ld16(o_cols(s) + lanes + c, o);
@@ -497,16 +517,16 @@ attention_tc_kernel(const __grid_constant__ TcAttnArgs t)
                 }
             }
         }
-        __syncthreads();
     } else {
-        __syncthreads();                                                // the other tile's products have read their operands too
-        float *rows = reinterpret_cast<float *>(smem_raw);
+        float *rows = reinterpret_cast<float *>(smem_raw), *tops = rows + 256 * C::PITCH, *sums = tops + 256;
         if (mine) {
-            sh->top[s * 128 + row] = top * t.scale_log2;
-            sh->sum[s * 128 + row] = sum;
-            if (tiles > 0 && ok) {
+            if (half == 0) {
+                tops[s * 128 + row] = top * t.scale_log2;
+                sums[s * 128 + row] = sum;
+            }
+            if (tiles > 0) {
 #pragma unroll 1
-                for (int c = 0; c < DP; c += 16) {
+                for (int c = o0; c < o1; c += 16) {
                     uint32_t o[16];
                     tmem_ld16(o_cols(s) + lanes + c, o);
                     tmem_ld_wait();
@@ -516,25 +536,16 @@ attention_tc_kernel(const __grid_constant__ TcAttnArgs t)
                 }
             }
         }
-        cluster_sync_all();
+        cluster_done();
         if (!*abort_flag)
-            join_rows<__nv_bfloat16>(smem_u32(rows), C::PITCH, smem_u32(sh->top), smem_u32(sh->sum), 128 * sides, a.d, rank, t.splits, tid, THREADS, [&](int r) -> __nv_bfloat16 * {
+            join_rows<__nv_bfloat16>(smem_u32(rows), C::PITCH, smem_u32(tops), smem_u32(sums), 128 * sides, a.d, rank, t.splits, tid, SOFT_WARPS * 32, [&](int r) -> __nv_bfloat16 * {
                 const int in_tile = r & 127, token = token0 + (r >> 7) * t.q_tokens + in_tile / a.group;
                 if (in_tile >= t.q_tokens * a.group || token >= a.lq) return nullptr;
                 return (__nv_bfloat16 *)a.y + ((size_t)image * a.lq + token) * a.yp + (kv_head * a.group + in_tile % a.group) * a.d;
             });
-        __syncwarp();
-        cluster_sync_all();                                             // a peer's rows are read until here
+        cluster_done();                                                 // a peer's rows are read until here
     }
-    if (*abort_flag) {                                                  // loads and products in flight end before their memory goes
-        const long long begin = clock64();
-        while (clock64() - begin < 4000000LL) { }
-    }
-    __syncthreads();
-    if (warp == 9) {
-        tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
-    }
+    finish();
 }
 
 typedef void (*Kernel)(TcAttnArgs);
@@ -563,7 +574,6 @@ int launch_attention_tc(const AttnArgs &a, cudaStream_t stream)
 {
     TcAttnArgs t;
     t.a = a;
-    if (!t.a.wait_limit) t.a.wait_limit = WAIT_LIMIT_CYCLES;
     t.q_tokens = 128 / a.group;
     t.q_tiles = (a.lq + 2 * t.q_tokens - 1) / (2 * t.q_tokens);
     t.scale_log2 = (a.scale < 0.f ? -a.scale : a.scale) * 1.4426950408889634f;
@@ -593,7 +603,7 @@ int launch_attention_tc(const AttnArgs &a, cudaStream_t stream)
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(jobs * t.splits));
     cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = tmem_smem((a.d > 64 ? Cfg<128>::WORK : Cfg<64>::WORK) + sizeof(Shared), 512);
+    cfg.dynamicSmemBytes = tmem_smem(a.d > 64 ? Cfg<128>::BYTES : Cfg<64>::BYTES, 512);
     cfg.stream = stream;
     cfg.attrs = attrs;
     cfg.numAttrs = 2;

@@ -112,6 +112,30 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     return ok != 0;
 }
 
+// Bounded wait for hand-overs of a microsecond or less: nothing but polls, counted, and the abort flag.  The waits above cost their callers 400 to 500
+// clocks a hand-over (the suspend hint, the clock, the code around them and the registers it holds); this one about 100.  It has no outcome: a wait that ran out
+// has set the abort flag, and whoever called it goes on over whatever is there, in bounds, every later wait of his a short one.
+__device__ __forceinline__ void mbar_wait_tight(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *status, int code, int polls)
+{
+    int n = 0;
+    while (!mbar_try_wait(bar, parity)) {
+        if (*abort_flag) break;
+        if (++n > polls) {
+            *abort_flag = 1;
+            atomicCAS(status, 0, code);
+            break;
+        }
+    }
+    __syncwarp();
+}
+// The same of a warp that has to know: a loader, or one that issues products, stops at a wait that ran out.
+__device__ __forceinline__ bool mbar_wait_known(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *status, int code, int polls)
+{
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    mbar_wait_tight(bar, parity, abort_flag, status, code, polls);
+    return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) && !__any_sync(0xffffffffu, *abort_flag != 0);
+}
+
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1, int c2, int c3)
 {
     asm volatile(
