@@ -13,19 +13,39 @@ from . import (ACTIVATIONS, BF16, E4M3, F32, MODE_TF32, NCHW, NHWC, AttentionDes
 
 
 _current = None
+_functions = {}
+_torch = None
 
 
-def _stream(stream=None) -> C.c_void_p:
-    """The stream a call goes to: the caller's, or torch's current one.  torch.cuda.current_stream() makes a Python object of it, 3.2 us of the 8.5
-    that the smallest call takes its host; torch's own handle of it is there in 0.2."""
+def _types():
+    """torch, imported at its first use."""
+    global _torch
+    if _torch is None:
+        import torch
+        _torch = torch
+    return _torch
+
+
+def _stream(stream=None):
+    """The stream a call goes to, as a number: the caller's, or torch's current one.  torch.cuda.current_stream() makes a Python object of it, 3.2 us of the
+    8.5 that the smallest call takes its host; torch's own handle of it is there in 0.2."""
     global _current
     if stream is not None:
-        return C.c_void_p(int(stream))
+        return int(stream)
     if _current is None:
         import torch
-        raw, device = getattr(torch._C, "_cuda_getCurrentRawStream", None), torch.cuda.current_device
+        torch.cuda.current_device()                   # torch's first use of the device
+        raw, device = getattr(torch._C, "_cuda_getCurrentRawStream", None), getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
         _current = (lambda: raw(device())) if raw else (lambda: torch.cuda.current_stream().cuda_stream)
-    return C.c_void_p(_current())
+    return _current()
+
+
+def _function(name):
+    """A function of the library, looked up once: the calls of a few microseconds go through here."""
+    f = _functions.get(name)
+    if f is None:
+        f = _functions[name] = getattr(lib(), name)
+    return f
 
 
 def as_tensor(t, layout: int = NCHW, c: int | None = None) -> Tensor:
@@ -143,7 +163,7 @@ def softmax(x: Tensor, y: Tensor, groups: int = 1, temperature: float = 1.0, str
 
 def _device_array(t, dtypes, shape, what):
     """The address of a contiguous CUDA tensor of one of `dtypes` and of `shape`."""
-    if not t.is_cuda or t.dtype not in dtypes or tuple(t.shape) != shape or not t.is_contiguous():
+    if not t.is_cuda or t.dtype not in dtypes or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{what}: needs a contiguous CUDA tensor {list(shape)} of {' or '.join(str(d) for d in dtypes)}")
     return t.data_ptr()
 
@@ -164,9 +184,10 @@ class RopePlan:
     def forward(self, x: Tensor, y: Tensor, positions=None, stream=None):
         """positions: int32 CUDA torch tensor [n * h * w, 3], or None for the tokens' places in the map."""
         if positions is not None:
-            import torch
-            positions = _device_array(positions, (torch.int32,), (x.n * x.h * x.w, 3), "positions")
-        check(lib().dnb_rope_forward(self.handle, C.byref(x), positions, C.byref(y), _stream(stream)))
+            positions = _device_array(positions, (_types().int32,), (x.n * x.h * x.w, 3), "positions")
+        status = _function("dnb_rope_forward")(self.handle, C.byref(x), positions, C.byref(y), _stream(stream))
+        if status:
+            check(status)
 
     def close(self):
         if self.handle:
@@ -193,17 +214,18 @@ class CrossAttentionPlan:
         expanded along images and queries."""
         masks = None
         if lengths is not None or mask is not None:
-            import torch
             masks = AttentionMask(None, None, 0, 0)
             if lengths is not None:
-                masks.lengths = _device_array(lengths, (torch.int32,), (q.n,), "lengths")
+                masks.lengths = _device_array(lengths, (_types().int32,), (q.n,), "lengths")
             if mask is not None:
                 keys = k.h * k.w
-                if not mask.is_cuda or mask.dtype not in (torch.bool, torch.uint8) or tuple(mask.shape) != (q.n, q.h * q.w, keys) or (keys > 1 and mask.stride(2) != 1):
+                if not mask.is_cuda or mask.dtype not in (_types().bool, _types().uint8) or mask.shape != (q.n, q.h * q.w, keys) or (keys > 1 and mask.stride(2) != 1):
                     raise ValueError(f"mask: needs a CUDA tensor [{q.n}, {q.h * q.w}, {keys}] of bool or uint8 with contiguous keys")
                 masks.mask, masks.image_stride, masks.query_stride = mask.data_ptr(), mask.stride(0), mask.stride(1)
             masks = C.byref(masks)
-        check(lib().dnb_attention_forward(self.handle, C.byref(q), C.byref(k), C.byref(v), masks, C.byref(y), _stream(stream)))
+        status = _function("dnb_attention_forward")(self.handle, C.byref(q), C.byref(k), C.byref(v), masks, C.byref(y), _stream(stream))
+        if status:
+            check(status)
 
     @property
     def kernel(self) -> str:
@@ -235,15 +257,15 @@ def rmsnorm(x: Tensor, y: Tensor | None = None, gain=None, eps=1e-6, residual: T
     gain: float32 CUDA torch tensor [c].  e4m3: float8_e4m3fn (or uint8) CUDA torch tensor [n, h, w, pitch] with scales, a float32 one
     [n, h, w, groups]; group: channels that share a scale (32, 64, 128), or 0 for all."""
     q = None
-    if gain is not None or e4m3 is not None:
-        import torch
-        if gain is not None:
-            gain = _device_array(gain, (torch.float32,), (x.c,), "gain")
-        if e4m3 is not None:
-            pitch = e4m3.shape[-1]
-            data = _device_array(e4m3, (torch.float8_e4m3fn, torch.uint8), (x.n, x.h, x.w, pitch), "e4m3")
-            q = C.byref(E4M3(data, _device_array(scales, (torch.float32,), (x.n, x.h, x.w, -(-x.c // group) if group > 0 else 1), "scales"), pitch, group))
-    check(lib().dnb_rmsnorm_forward(C.byref(x), _ref(residual), gain, eps, _ref(total), _ref(y), q, _stream(stream)))
+    if gain is not None:
+        gain = _device_array(gain, (_types().float32,), (x.c,), "gain")
+    if e4m3 is not None:
+        pitch = e4m3.shape[-1]
+        data = _device_array(e4m3, (_types().float8_e4m3fn, _types().uint8), (x.n, x.h, x.w, pitch), "e4m3")
+        q = C.byref(E4M3(data, _device_array(scales, (_types().float32,), (x.n, x.h, x.w, -(-x.c // group) if group > 0 else 1), "scales"), pitch, group))
+    status = _function("dnb_rmsnorm_forward")(C.byref(x), _ref(residual), gain, eps, _ref(total), _ref(y), q, _stream(stream))
+    if status:
+        check(status)
 
 
 class Network:

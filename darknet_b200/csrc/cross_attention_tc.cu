@@ -367,21 +367,23 @@ attention_tc_kernel(const __grid_constant__ TcAttnArgs t)
             const int key0 = (t0 + j) * 128, left = keys - key0, col0 = half * 64;
             uint32_t bits[2] = {0xffffffffu, 0xffffffffu};
             if (MASK) {
-                // The rows' masks, one row after another, 32 keys a load; rows of one query (heads that share keys) share the load.
-                const uint8_t *last = nullptr;
-                uint32_t now[2] = {0, 0};
-                for (int i = 0; i < 32; ++i) {
-                    const uint8_t *p = reinterpret_cast<const uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mask), i));
-                    if (p != last) {
-                        last = p;
-                        p += key0 + col0;
+                // The rows' masks, 32 keys of a row a load, sixteen rows' loads in flight together; one row's where all are alike.
+                const int rows = a.mask_query == 0 ? 1 : 32;
+                for (int i0 = 0; i0 < rows; i0 += 16) {
+                    uint8_t m[16][2];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const uint8_t *p = reinterpret_cast<const uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mask), i0 + i)) + key0 + col0;
+#pragma unroll
+                        for (int w = 0; w < 2; ++w) m[i][w] = i0 + i < rows && col0 + lane + 32 * w < left ? p[lane + 32 * w] : 0;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
 #pragma unroll
                         for (int w = 0; w < 2; ++w) {
-                            const int c = lane + 32 * w;
-                            now[w] = __ballot_sync(0xffffffffu, col0 + c < left && p[c] != 0);
+                            const uint32_t now = __ballot_sync(0xffffffffu, m[i][w] != 0);
+                            if (rows == 1 ? i == 0 : lane == i0 + i) bits[w] = now;
                         }
-                    }
-                    if (lane == i) { bits[0] = now[0]; bits[1] = now[1]; }
                 }
             } else if (left < 128) {
 #pragma unroll

@@ -82,8 +82,17 @@ rmsnorm_kernel(const __grid_constant__ NormArgs a)
     launch_dependents_if_small();
     const float per_channel = 1.f / (float)a.c;
     uint64_t gain[VECS][P::N];
+    const bool wide = a.gain && (uintptr_t)a.gain % 16 == 0;
 #pragma unroll
     for (int k = 0; k < VECS; ++k)
+        if (wide && (WHOLE || (lane + k * LANES) * N + N <= a.c)) {
+#pragma unroll
+            for (int e = 0; e < P::N; e += 2) {
+                const float4 g = __ldg(reinterpret_cast<const float4 *>(a.gain + (lane + k * LANES) * N + 2 * e));
+                gain[k][e] = pack2(g.x, g.y);
+                gain[k][e + 1] = pack2(g.z, g.w);
+            }
+        } else
 #pragma unroll
         for (int e = 0; e < P::N; ++e) {
             const int ch = (lane + k * LANES) * N + 2 * e;

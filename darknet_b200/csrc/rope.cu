@@ -5,7 +5,7 @@
 //
 // Angles: sine and cosine want t modulo a turn.  A float of t loses that for far positions (position 1e5 has 1/128 of a radian between neighbours),
 // so the angle is position * F modulo 2^64, where F is the pair's scale * frequency / 2 pi, its whole turns dropped, in units of 2^-64 turns:
-// one integer product, exact modulo a turn, off by at most position * 2^-65 turns however far the position is.
+// one integer product, exact modulo a turn, off by at most position * 2^-62 turns (2^-31 for the last position) however far the position is.
 #include <math.h>
 #include <string.h>
 
@@ -18,8 +18,7 @@
 struct dnb_rope_plan {
     dnb_rope_desc d;
     int pairs;                             // P, over all axes
-    uint64_t turn[DNB_ROPE_MAX_PAIRS];     // F of each pair
-    uint8_t axis[DNB_ROPE_MAX_PAIRS];
+    uint64_t turn[DNB_ROPE_MAX_PAIRS];     // F of each pair, its last two bits the axis
 };
 
 namespace dnb {
@@ -28,7 +27,6 @@ constexpr int ROPE_THREADS = 128;
 
 struct RopeArgs {
     uint64_t turn[DNB_ROPE_MAX_PAIRS];
-    uint8_t axis[DNB_ROPE_MAX_PAIRS];
     const void *x;
     void *y;
     const int32_t *positions;              // [tokens][3], or null: the token's place
@@ -40,6 +38,20 @@ struct RopeArgs {
     int chunk, chunks;                     // heads of a thread, and how many such shares a token has
     unsigned turners;                      // blocks that turn; the blocks behind them copy what passes
 };
+
+// Sine and cosine of turns * 2^-32 of a turn: the nearest quarter taken off in whole numbers, polynomials of the rest's angle (at most pi / 4) fitted to the
+// smallest largest error (4e-09 of the sine, 1e-10 of the cosine, before rounding).
+__device__ __forceinline__ void sine_of(int turns, float &s, float &c)
+{
+    const int quarter = (int)((unsigned)turns + (1u << 29)) >> 30;
+    const float x = (float)(int)((unsigned)turns - ((unsigned)quarter << 30)) * (6.283185307179586f * 0x1p-32f), z = x * x;
+    const float sine = fmaf(x * z, fmaf(z, fmaf(z, -0.0001951729936990887f, 0.008332177996635437f), -0.16666655242443085f), x);
+    const float cosine = fmaf(z, fmaf(z, fmaf(z, fmaf(z, 2.4438451873720624e-05f, -0.001388736767694354f), 0.04166664555668831f), -0.5f), 1.f);
+    s = quarter & 1 ? cosine : sine;
+    c = quarter & 1 ? sine : cosine;
+    if (quarter & 2) s = -s;
+    if ((quarter + 1) & 2) c = -c;
+}
 
 template <int BYTES> struct RopeVec;
 template <> struct RopeVec<2> { using type = uint16_t; };
@@ -62,16 +74,25 @@ rope_kernel(const __grid_constant__ RopeArgs a)
     T *y = (T *)a.y;
     const int per_head = a.pairs / V;
     if (blockIdx.x < a.turners) {
-        __shared__ uint64_t turn[DNB_ROPE_MAX_PAIRS];                             // threads read them in many orders, constants in one
-        __shared__ uint8_t axis[DNB_ROPE_MAX_PAIRS];
-        for (int i = threadIdx.x; i < a.pairs; i += ROPE_THREADS) { turn[i] = a.turn[i]; axis[i] = a.axis[i]; }
-        __syncthreads();
         const unsigned long long item = (unsigned long long)blockIdx.x * ROPE_THREADS + threadIdx.x;
-        const unsigned part = (unsigned)(item / (unsigned)per_head);              // fits: tokens * chunks < 2^31
+        const unsigned part = item >> 32 ? (unsigned)(item / (unsigned)per_head) : (unsigned)item / (unsigned)per_head;   // fits: tokens * chunks < 2^31
         const int j = (int)(item - (unsigned long long)part * (unsigned)per_head) * V;
         const unsigned token = part / (unsigned)a.chunks;
         const int head0 = (int)(part - token * (unsigned)a.chunks) * a.chunk;
         if (token >= a.tokens) return;
+        const int at_a = INTERLEAVED ? 2 * j : j, apart = INTERLEAVED ? V : a.pairs, count = min(a.chunk, a.heads - head0);
+        const T *src = x + (size_t)token * a.xp + head0 * a.head_dim + at_a;
+        T *dst = y + (size_t)token * a.yp + head0 * a.head_dim + at_a;
+        Vec va[AT_ONCE], vb[AT_ONCE];
+        auto load = [&](int h0) {
+#pragma unroll
+            for (int h = 0; h < AT_ONCE; ++h)
+                if (h0 + h < count) {
+                    va[h].raw = *reinterpret_cast<const Raw *>(src + h * a.head_dim);
+                    vb[h].raw = *reinterpret_cast<const Raw *>(src + h * a.head_dim + apart);
+                }
+        };
+        load(0);                                                                  // on their way while the sines are worked out
         long long at[3];
         if (a.positions) {
 #pragma unroll
@@ -85,24 +106,16 @@ rope_kernel(const __grid_constant__ RopeArgs a)
         float cs[V], sn[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            const int s = axis[j + e];
+            const uint64_t turn = a.turn[j + e];
+            const int s = (int)(turn & 3);
             const uint64_t where = (uint64_t)(s == 0 ? at[0] : s == 1 ? at[1] : at[2]);
-            const int turns = (int)(where * turn[j + e] >> 32);                   // signed: from -1/2 to 1/2 of a turn, in units of 2^-32
+            const int turns = (int)(where * turn >> 32);                          // signed: from -1/2 to 1/2 of a turn, in units of 2^-32
             // bf16: the hardware's sine, off by 2^-21.4 at most on one turn, where half a step of the output is 2^-9 or more of it
             if (sizeof(T) == 2) __sincosf((float)turns * (6.283185307179586f * 0x1p-32f), &sn[e], &cs[e]);
-            else sincospif((float)turns * 0x1p-31f, &sn[e], &cs[e]);
+            else sine_of(turns, sn[e], cs[e]);
         }
-        const int at_a = INTERLEAVED ? 2 * j : j, apart = INTERLEAVED ? V : a.pairs, count = min(a.chunk, a.heads - head0);
-        const T *src = x + (size_t)token * a.xp + head0 * a.head_dim + at_a;
-        T *dst = y + (size_t)token * a.yp + head0 * a.head_dim + at_a;
         for (int h0 = 0; h0 < count; h0 += AT_ONCE, src += AT_ONCE * a.head_dim, dst += AT_ONCE * a.head_dim) {
-            Vec va[AT_ONCE], vb[AT_ONCE];
-#pragma unroll
-            for (int h = 0; h < AT_ONCE; ++h)
-                if (h0 + h < count) {
-                    va[h].raw = *reinterpret_cast<const Raw *>(src + h * a.head_dim);
-                    vb[h].raw = *reinterpret_cast<const Raw *>(src + h * a.head_dim + apart);
-                }
+            if (h0) load(h0);
 #pragma unroll
             for (int h = 0; h < AT_ONCE; ++h)
                 if (h0 + h < count) {
@@ -172,7 +185,6 @@ static int launch_rope(const dnb_rope_plan &p, const dnb_tensor *x, const int32_
     if ((long long)x->n * x->h >= 1LL << 31 || tokens >= 1LL << 31) DNB_FAIL(DNB_EUNSUPPORTED, "rope: 2^31 tokens or more");
     RopeArgs a;
     memcpy(a.turn, p.turn, sizeof(a.turn));
-    memcpy(a.axis, p.axis, sizeof(a.axis));
     a.x = x->data; a.y = y->data; a.positions = positions;
     a.tokens = (unsigned)tokens;
     a.xp = x->cpitch; a.yp = y->cpitch;
@@ -183,10 +195,12 @@ static int launch_rope(const dnb_rope_plan &p, const dnb_tensor *x, const int32_
     // the widest vector that the pairs and the heads are whole numbers of
     int v = x->dtype == DNB_BF16 ? 8 : 4;
     while (p.pairs % v || d.head_dim % v) v /= 2;
-    // Heads of a thread: eight, so that its sines cost it little; fewer while there are too few threads to fill the GPU.
+    // Heads of a thread: eight, so that its sines cost it little; fewer while the GPU has room for the threads, two blocks an SM (a grid of that size starts
+    // early, see launch_overlapped).
     const int per_head = p.pairs / v;
+    auto threads = [&](int chunk) { return tokens * per_head * ((d.heads + chunk - 1) / chunk); };
     a.chunk = d.heads < 8 ? d.heads : 8;
-    while (a.chunk > 1 && tokens * per_head * ((d.heads + a.chunk - 1) / a.chunk) < (long long)sm_count() * 1024) a.chunk = (a.chunk + 1) / 2;
+    while (a.chunk > 1 && threads((a.chunk + 1) / 2) <= (long long)sm_count() * 2 * ROPE_THREADS) a.chunk = (a.chunk + 1) / 2;
     a.chunks = (d.heads + a.chunk - 1) / a.chunk;
     if (tokens * a.chunks >= 1LL << 31) { a.chunk = d.heads; a.chunks = 1; }
     const unsigned long long turners = ((unsigned long long)tokens * a.chunks * per_head + ROPE_THREADS - 1) / ROPE_THREADS;
@@ -239,8 +253,7 @@ extern "C" int dnb_rope_plan_create(const dnb_rope_desc *desc, dnb_rope_plan **p
             const long double power = d.shared ? (long double)i / pairs : (long double)j / d.pairs[axis];
             const long double per_step = powl((long double)d.base, -power) * d.scale[axis] / (2 * 3.141592653589793238462643383279502884L);
             const long double turn = per_step - floorl(per_step);                 // 0 <= turn < 1 (1 if it rounds up)
-            p->turn[i] = turn * 0x1p64L >= 0x1p64L ? 0 : (uint64_t)(turn * 0x1p64L);
-            p->axis[i] = (uint8_t)axis;
+            p->turn[i] = ((turn * 0x1p64L >= 0x1p64L ? 0 : (uint64_t)(turn * 0x1p64L)) & ~3ULL) | (uint64_t)axis;
         }
     *plan = p;
     return DNB_OK;
