@@ -44,4 +44,8 @@ int launch_attention_rows(const AttnArgs &a, cudaStream_t s);
 bool attention_f32_covers(const AttnArgs &a, int dtype);
 int launch_attention_f32(const AttnArgs &a, cudaStream_t s);
 
+// ---- cross_attention_f32_tc.cu : f32, on the tensor cores
+bool attention_f32_tc_covers(const AttnArgs &a, int dtype);
+int launch_attention_f32_tc(const AttnArgs &a, cudaStream_t s);
+
 }  // namespace dnb

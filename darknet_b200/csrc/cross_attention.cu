@@ -175,6 +175,10 @@ extern "C" int dnb_attention_forward(dnb_attention_plan *p, const dnb_tensor *q,
         p->kernel = "rows_bf16";
         return launch_attention_rows(a, (cudaStream_t)stream);
     }
+    if (attention_f32_tc_covers(a, q->dtype) && (long long)a.lq * a.group > 16) {
+        p->kernel = "tc_f32";
+        return launch_attention_f32_tc(a, (cudaStream_t)stream);
+    }
     if (attention_f32_covers(a, q->dtype)) {
         p->kernel = "fma_f32";
         return launch_attention_f32(a, (cudaStream_t)stream);

@@ -68,7 +68,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t *r)
         ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
           "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
 }
-__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // Waits for the loads so far; the values pass through it, so that nothing that uses them is moved in front of it.
 __device__ __forceinline__ void tmem_ld_wait32(uint32_t *r)
 {
@@ -77,13 +76,6 @@ __device__ __forceinline__ void tmem_ld_wait32(uint32_t *r)
                    "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
                    "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
 }
-__device__ __forceinline__ float max3_nan(float a, float b, float c)
-{
-    float r;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
-
 // V as it lies in shared memory: rows of 64 channels (128 bytes, swizzled), a key each: N is contiguous.  Blocks of 64 channels are a box
 // apart, groups of eight keys 1024 bytes.
 __device__ __forceinline__ uint64_t desc_values(uint32_t addr)
@@ -95,21 +87,6 @@ __device__ __forceinline__ uint64_t desc_values(uint32_t addr)
     d |= (uint64_t)2 << 61;
     return d;
 }
-template <bool ADD>
-__device__ __forceinline__ void umma_from_tmem(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate)
-{
-    if (ADD)
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.eq.b32 p, 0, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-            ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc) : "memory");
-    else
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-            ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
-}
-
 // DP: channels of a head as they lie in shared memory, 64 or 128 (TMA fills what the head does not have with zeros).
 template <int DP> struct Cfg {
     static constexpr int BOXES = DP / 64;

@@ -329,7 +329,9 @@ void dnb_attention_plan_destroy(dnb_attention_plan *plan);
 /* y = softmax(scale q k^T) v.  q, y: [n][..][heads * head_dim]; k, v: [n or 1][..][kv_heads * head_dim], one image of
  * states for all of q's where it is 1.  mask may be NULL.  A query that sees no key gets zeros.  y is no input's
  * memory.  Keys and values at and behind an image's length are not used, whatever they hold, and nor are those that a
- * mask with query_stride 0 hides; with a mask for each query, what only some of them may see has to be finite in v. */
+ * mask with query_stride 0 hides; with a mask for each query, what only some of them may see has to be finite in v.
+ * f32 operands are multiplied as sums of three bf16 numbers where a key head has more than 16 rows: an infinity, or a
+ * number beyond bf16's largest (3.39e38), that a query sees makes NaN of the outputs that it reaches. */
 int dnb_attention_forward(dnb_attention_plan *plan, const dnb_tensor *q, const dnb_tensor *k, const dnb_tensor *v,
                           const dnb_attention_mask *mask, const dnb_tensor *y, void *stream);
 
