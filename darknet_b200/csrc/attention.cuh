@@ -23,6 +23,18 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c)
     return r;
 }
 
+// Two floats as three pairs of bf16, each the nearest of what is left.
+__device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &mid, uint32_t &lo)
+{
+    hi = pack_bf16(x, y);
+    x -= __uint_as_float(hi << 16);
+    y -= __uint_as_float(hi & 0xffff0000u);
+    mid = pack_bf16(x, y);
+    x -= __uint_as_float(mid << 16);
+    y -= __uint_as_float(mid & 0xffff0000u);
+    lo = pack_bf16(x, y);
+}
+
 // An MMA whose A lies in TMEM: the weights.  ADD: onto the sums so far, whatever `accumulate` says.
 template <bool ADD>
 __device__ __forceinline__ void umma_from_tmem(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate)

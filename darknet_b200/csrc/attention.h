@@ -36,13 +36,9 @@ int launch_attention_simple(const AttnArgs &a, int dtype, cudaStream_t s);
 bool attention_tc_covers(const AttnArgs &a, int dtype);
 int launch_attention_tc(const AttnArgs &a, cudaStream_t s);
 
-// ---- cross_attention_rows.cu : bf16, up to 16 rows a key head
-bool attention_rows_covers(const AttnArgs &a, int dtype);
-int launch_attention_rows(const AttnArgs &a, cudaStream_t s);
-
-// ---- cross_attention_f32.cu : f32, on the CUDA cores
-bool attention_f32_covers(const AttnArgs &a, int dtype);
-int launch_attention_f32(const AttnArgs &a, cudaStream_t s);
+// ---- cross_attention_rows.cu : up to 16 rows a key head
+bool attention_rows_covers(const AttnArgs &a);
+int launch_attention_rows(const AttnArgs &a, int dtype, cudaStream_t s);
 
 // ---- cross_attention_f32_tc.cu : f32, on the tensor cores
 bool attention_f32_tc_covers(const AttnArgs &a, int dtype);

@@ -171,17 +171,13 @@ extern "C" int dnb_attention_forward(dnb_attention_plan *p, const dnb_tensor *q,
     a.polls = polls > 0x7fffffff ? 0x7fffffff : (int)polls;
     if (p->device < 0) DNB_FAIL(DNB_ECUDA, "attention: the plan was made without a CUDA device");
     DNB_TRY(check_current_device(p->device, "attention"));
-    if (attention_rows_covers(a, q->dtype)) {
-        p->kernel = "rows_bf16";
-        return launch_attention_rows(a, (cudaStream_t)stream);
+    if (attention_rows_covers(a)) {
+        p->kernel = q->dtype == DNB_F32 ? "rows_f32" : "rows_bf16";
+        return launch_attention_rows(a, q->dtype, (cudaStream_t)stream);
     }
-    if (attention_f32_tc_covers(a, q->dtype) && (long long)a.lq * a.group > 16) {
+    if (attention_f32_tc_covers(a, q->dtype)) {
         p->kernel = "tc_f32";
         return launch_attention_f32_tc(a, (cudaStream_t)stream);
-    }
-    if (attention_f32_covers(a, q->dtype)) {
-        p->kernel = "fma_f32";
-        return launch_attention_f32(a, (cudaStream_t)stream);
     }
     if (attention_tc_covers(a, q->dtype)) {
         p->kernel = "tc_bf16";

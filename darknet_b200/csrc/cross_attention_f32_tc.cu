@@ -48,18 +48,6 @@ template <int DP> struct F32TcCfg {
     static_assert(130 * PITCH * 4 <= (int)WORK && BYTES <= 232448, "fits an SM");
 };
 
-// Two floats as three pairs of bf16, each the nearest of what is left.
-__device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &mid, uint32_t &lo)
-{
-    hi = pack_bf16(x, y);
-    x -= __uint_as_float(hi << 16);
-    y -= __uint_as_float(hi & 0xffff0000u);
-    mid = pack_bf16(x, y);
-    x -= __uint_as_float(mid << 16);
-    y -= __uint_as_float(mid & 0xffff0000u);
-    lo = pack_bf16(x, y);
-}
-
 // Eight channels of row r, channels 8c .., in three parts to their swizzled places.
 __device__ __forceinline__ void store_parts(uint8_t *base, uint32_t box, uint32_t part, int r, int c, const float4 &x, const float4 &y)
 {

@@ -1,9 +1,14 @@
-// Cross attention of bf16 tensors for few query rows a key head: single tokens, and the query heads that share its keys.
+// Cross attention for few query rows a key head: single tokens, and the query heads that share its keys.
 //
 // The bytes of keys and values bound it: each is read once, by TMA, through a ring of tiles of 64 keys that keeps about 100 KB an SM's block (two of
 // them an SM) on the way.  Four warps, 16 keys of a tile each, multiply them by up to 16 rows with mma.sync: the 128 rows of a tcgen05 product would be
 // empty but for a few, its TMEM round trip is a latency for each tile, and the arithmetic is far from any bound either way.  A warp has a running maximum
 // and sum of its own keys; warps, and the CTAs of a cluster that share the keys of one head, meet once at the end.
+//
+// f32 operands are sums of three bf16 numbers (24 bits of mantissa), their product the six products of parts that reach 2^-24 of it, smallest first; a tile's
+// sums are added to the rows' in fp32, since the tensor cores' sums lose a little at each addition.  A lane reads four channels of a key at once: which
+// channel of the head stands where along a product's K, and which key or channel along its N, is free as long as both operands agree, and is chosen
+// such that the eight lanes of a 16-byte load meet all banks.
 #include <atomic>
 
 #include "attention.cuh"
@@ -17,12 +22,14 @@ namespace {
 constexpr int R_KEYS = 64, R_WARPS = 4, R_THREADS = R_WARPS * 32 + 32;
 constexpr float R_MOVE = 8.f;                     // how far (log2) scores may outgrow the running maximum before the sums are corrected
 
-template <int DP> struct RowsCfg {
-    static constexpr int BOXES = DP / 64;
+template <typename T, int DP> struct RowsCfg {
+    static constexpr bool F32 = sizeof(T) == 4;
+    static constexpr int BOX_CHANNELS = 128 / sizeof(T), BOXES = DP / BOX_CHANNELS;
     static constexpr uint32_t BOX = R_KEYS * 128, TILE = BOXES * BOX;
-    static constexpr int STAGES = DP == 128 ? 6 : 12;
+    static constexpr int STAGES = 12 / BOXES;
     static constexpr int PITCH = DP + 4;
-    static constexpr uint32_t WORK = STAGES * TILE;
+    static constexpr uint32_t WORK = STAGES * TILE, Q_PART = DP / 16 * 512;    // Q_PART: fragments of one part of the queries, f32 only
+    static constexpr uint32_t BYTES = WORK + (F32 ? 3 * Q_PART : 0);           // in front of RowsShared
     static_assert((R_WARPS + 1) * 16 * PITCH * 4 <= (int)WORK, "the warps' sums fit where the tiles were");
 };
 
@@ -53,11 +60,11 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <int DP>
+template <typename T, int DP>
 __global__ void __launch_bounds__(R_THREADS, 2)
 attention_rows_kernel(const __grid_constant__ RowsArgs t)
 {
-    using C = RowsCfg<DP>;
+    using C = RowsCfg<T, DP>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const AttnArgs &a = t.a;
     const uint32_t ring = smem_u32(smem_raw);
@@ -65,7 +72,7 @@ attention_rows_kernel(const __grid_constant__ RowsArgs t)
         if (threadIdx.x == 0) atomicCAS(a.status, 0, AT_SMEM_BASE);
         return;
     }
-    RowsShared *sh = reinterpret_cast<RowsShared *>(smem_raw + C::WORK);
+    RowsShared *sh = reinterpret_cast<RowsShared *>(smem_raw + C::BYTES);
     volatile int *abort_flag = &sh->abort_flag;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int rank = (int)(blockIdx.x % (unsigned)t.splits), job = (int)(blockIdx.x / (unsigned)t.splits);
@@ -87,6 +94,7 @@ attention_rows_kernel(const __grid_constant__ RowsArgs t)
     int keys = a.lk, first, tiles;
     if (a.lengths) keys = min(max(a.lengths[image], 0), a.lk);
     share_of_keys(keys, R_KEYS, rank, t.splits, first, tiles);
+    const int boxes = C::F32 ? (a.d + C::BOX_CHANNELS - 1) / C::BOX_CHANNELS : C::BOXES;     // that hold channels of the head
     // the token and head of row r: where its channels start in q (and, with y's pitch, in y)
     auto q_at = [&](int r, int pitch) { return ((size_t)image * a.lq + r / a.group) * pitch + (kv_head * a.group + r % a.group) * a.d; };
 
@@ -97,9 +105,9 @@ attention_rows_kernel(const __grid_constant__ RowsArgs t)
             const uint32_t full = smem_u32(&sh->full[stage]);
             if (!mbar_wait_known(smem_u32(&sh->empty[stage]), phase ^ 1, abort_flag, a.status, AT_SLOT, a.polls)) break;
             if (elect_one() && !(a.debug & 32 && i == 1)) {
-                mbar_expect_tx(full, C::TILE);
-                for (int b = 0; b < C::BOXES; ++b)
-                    tma_load_4d(ring + stage * C::TILE + b * C::BOX, i & 1 ? &t.tmv : &t.tmk, full, b * 64, kv_head, (first + i / 2) * R_KEYS, a.kn == 1 ? 0 : image);
+                mbar_expect_tx(full, boxes * C::BOX);
+                for (int b = 0; b < boxes; ++b)
+                    tma_load_4d(ring + stage * C::TILE + b * C::BOX, i & 1 ? &t.tmv : &t.tmk, full, b * C::BOX_CHANNELS, kv_head, (first + i / 2) * R_KEYS, a.kn == 1 ? 0 : image);
             }
             if (++stage == C::STAGES) { stage = 0; phase ^= 1; }
         }
@@ -108,15 +116,36 @@ attention_rows_kernel(const __grid_constant__ RowsArgs t)
 
     const int g = lane >> 2, c2 = (lane & 3) * 2;                       // this lane's rows g and g + 8 of a product, columns c2 and c2 + 1
     float o[DP / 8][4] = {}, top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+    const uint4 *q_parts = reinterpret_cast<const uint4 *>(smem_raw + C::WORK) + lane;
     if (warp < R_WARPS && tiles > 0) {
-        uint32_t q[DP / 16][4];
+        if constexpr (C::F32) {
+            // the queries' fragments in three parts, the same for every warp: along K, channels 4 t .. 4 t + 3 of 16 stand at 2 t, 2 t + 1, 2 t + 8, 2 t + 9 (t = lane % 4)
+            for (int i = warp; i < DP / 16; i += R_WARPS) {
+                float4 x[2];
 #pragma unroll
-        for (int i = 0; i < DP / 16; ++i)
+                for (int e = 0; e < 2; ++e) {
+                    const int r = g + e * 8, c = i * 16 + 2 * c2;
+                    x[e] = r < rows && c < a.d ? *reinterpret_cast<const float4 *>((const float *)a.q + q_at(r, a.qp) + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+                uint4 f[3];
+                split2(x[0].x, x[0].y, f[0].x, f[1].x, f[2].x);
+                split2(x[1].x, x[1].y, f[0].y, f[1].y, f[2].y);
+                split2(x[0].z, x[0].w, f[0].z, f[1].z, f[2].z);
+                split2(x[1].z, x[1].w, f[0].w, f[1].w, f[2].w);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int r = g + (e & 1) * 8, c = i * 16 + c2 + (e >> 1) * 8;
-                q[i][e] = r < rows && c < a.d ? *reinterpret_cast<const uint32_t *>((const __nv_bfloat16 *)a.q + q_at(r, a.qp) + c) : 0u;
+                for (int p = 0; p < 3; ++p) *reinterpret_cast<uint4 *>(smem_raw + C::WORK + p * C::Q_PART + i * 512 + lane * 16) = f[p];
             }
+            asm volatile("bar.sync 1, %0;" ::"n"(R_WARPS * 32) : "memory");     // not with the warp that loads
+        }
+        uint32_t q[C::F32 ? 1 : DP / 16][4];
+        if constexpr (!C::F32)
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = g + (e & 1) * 8, c = i * 16 + c2 + (e >> 1) * 8;
+                    q[i][e] = r < rows && c < a.d ? *reinterpret_cast<const uint32_t *>((const __nv_bfloat16 *)a.q + q_at(r, a.qp) + c) : 0u;
+                }
         const uint8_t *mask[2] = {nullptr, nullptr};
         if (a.mask)
             for (int e = 0; e < 2; ++e) mask[e] = a.mask + (long long)image * a.mask_image + (long long)(g + e * 8 < rows ? (g + e * 8) / a.group : 0) * a.mask_query;
@@ -126,17 +155,46 @@ attention_rows_kernel(const __grid_constant__ RowsArgs t)
         auto next = [&]() { if (++stage == C::STAGES) { stage = 0; phase ^= 1; } };
         for (int j = 0; j < tiles; ++j) {
             const int key0 = (first + j) * R_KEYS + warp * 16, left = keys - key0;
-            bool in[2][4];                                              // row e, keys c2, c2 + 1, 8 + c2, 8 + c2 + 1
+            bool in[2][4];                                              // row e, keys c2, c2 + 1, 8 + c2, 8 + c2 + 1; of f32: t, t + 4, t + 8, t + 12
 #pragma unroll
             for (int e = 0; e < 2; ++e)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int key = (i >> 1) * 8 + c2 + (i & 1);
+                    const int key = C::F32 ? (lane & 3) + 4 * i : (i >> 1) * 8 + c2 + (i & 1);
                     in[e][i] = key < left && (!a.mask || mask[e][key0 + key]);
                 }
             mbar_wait_tight(smem_u32(&sh->full[stage]), phase, abort_flag, a.status, AT_KEYS, a.polls);
             float s[2][4] = {};
-            {
+            if constexpr (C::F32) {
+                // keys along N: n is key (n & 1) * 4 + n / 2 of eight
+                const uint8_t *at = smem_raw + stage * C::TILE + (warp * 16 + (g & 1) * 4 + (g >> 1)) * 128;
+                const int turn = ((g & 1) * 4 + (g >> 1)) << 4;         // the swizzle of that row
+                float small[2][4] = {};                                 // the products of parts but the highest
+#pragma unroll
+                for (int i = 0; i < DP / 16; ++i) {
+                    if (i * 16 >= a.d) break;
+                    uint32_t f[3][4];
+#pragma unroll
+                    for (int p = 0; p < 3; ++p) *reinterpret_cast<uint4 *>(f[p]) = q_parts[p * (C::Q_PART / 16) + i * 32];
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        const float4 x = *reinterpret_cast<const float4 *>(at + (i >> 1) * C::BOX + n * 1024 + (((i & 1) * 64 + (lane & 3) * 16) ^ turn));
+                        uint32_t b[3][2];
+                        split2(x.x, x.y, b[0][0], b[1][0], b[2][0]);
+                        split2(x.z, x.w, b[0][1], b[1][1], b[2][1]);
+                        mma16816(small[n], f[2], b[0][0], b[0][1]);
+                        mma16816(small[n], f[0], b[2][0], b[2][1]);
+                        mma16816(small[n], f[1], b[1][0], b[1][1]);
+                        mma16816(small[n], f[1], b[0][0], b[0][1]);
+                        mma16816(small[n], f[0], b[1][0], b[1][1]);
+                        mma16816(s[n], f[0], b[0][0], b[0][1]);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[n][e] += small[n][e];
+            } else {
                 const int key = warp * 16 + (m >> 1) * 8 + mr;
                 const uint32_t at = ring + stage * C::TILE + key * 128;
 #pragma unroll
@@ -177,7 +235,7 @@ attention_rows_kernel(const __grid_constant__ RowsArgs t)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) o[i][e] *= shrink[e >> 1];
             }
-            uint32_t p[4];
+            uint32_t p[C::F32 ? 3 : 1][4];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const float base = top[e] == -INFINITY ? 0.f : top[e];
@@ -185,7 +243,8 @@ attention_rows_kernel(const __grid_constant__ RowsArgs t)
                 for (int i = 0; i < 2; ++i) {
                     const float x = ex2(s[i][e * 2] - base), z = ex2(s[i][e * 2 + 1] - base);
                     sum[e] += x + z;
-                    p[i * 2 + e] = pack_bf16(x, z);
+                    if constexpr (C::F32) split2(x, z, p[0][i * 2 + e], p[1][i * 2 + e], p[2][i * 2 + e]);
+                    else p[0][i * 2 + e] = pack_bf16(x, z);
                 }
             }
             mbar_wait_tight(smem_u32(&sh->full[stage]), phase, abort_flag, a.status, AT_VALUES, a.polls);
@@ -203,7 +262,33 @@ attention_rows_kernel(const __grid_constant__ RowsArgs t)
                 fence_async_smem();                                     // before the slot's next load
                 __syncwarp();
             }
-            {
+            if constexpr (C::F32) {
+                // channels along N: of a box of 32, product e's n is channel 4 * ((n & 1) * 4 + n / 2) + e
+                const uint8_t *at = smem_raw + v_tile + (warp * 16 + (lane & 3)) * 128;
+                const int chunk = ((g & 1) * 4 + (g >> 1)) ^ (lane & 3);  // keys t + 4 and t + 12: the chunk four further
+#pragma unroll
+                for (int b = 0; b < C::BOXES; ++b) {
+                    if (b * 32 >= a.d) break;
+                    float x[4][4];                                      // keys t, t + 4, t + 8, t + 12
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) *reinterpret_cast<float4 *>(x[k]) = *reinterpret_cast<const float4 *>(at + b * C::BOX + k * 512 + ((chunk ^ (k & 1) * 4) << 4));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        uint32_t w[3][2];
+                        split2(x[0][e], x[1][e], w[0][0], w[1][0], w[2][0]);
+                        split2(x[2][e], x[3][e], w[0][1], w[1][1], w[2][1]);
+                        float now[4] = {};
+                        mma16816(now, p[2], w[0][0], w[0][1]);
+                        mma16816(now, p[0], w[2][0], w[2][1]);
+                        mma16816(now, p[1], w[1][0], w[1][1]);
+                        mma16816(now, p[1], w[0][0], w[0][1]);
+                        mma16816(now, p[0], w[1][0], w[1][1]);
+                        mma16816(now, p[0], w[0][0], w[0][1]);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) o[b * 4 + e][k] += now[k];
+                    }
+                }
+            } else {
                 const int key = warp * 16 + (m & 1) * 8 + mr;
                 const uint32_t at = ring + v_tile + key * 128;
 #pragma unroll
@@ -211,8 +296,8 @@ attention_rows_kernel(const __grid_constant__ RowsArgs t)
                     const int c = i * 16 + (m >> 1) * 8;
                     uint32_t b[4];
                     ldsm4t(at + (c >> 6) * C::BOX + (((c & 63) * 2) ^ (mr << 4)), b);
-                    mma16816(o[2 * i], p, b[0], b[1]);
-                    mma16816(o[2 * i + 1], p, b[2], b[3]);
+                    mma16816(o[2 * i], p[0], b[0], b[1]);
+                    mma16816(o[2 * i + 1], p[0], b[2], b[3]);
                 }
             }
             __syncwarp();
@@ -232,7 +317,15 @@ attention_rows_kernel(const __grid_constant__ RowsArgs t)
         for (int e = 0; e < 2; ++e) {
             const int r = warp * 16 + g + e * 8;
             if ((lane & 3) == 0) { sh->top[r] = top[e]; sh->sum[r] = sum[e]; }
-            if (g + e * 8 < rows)
+            if (g + e * 8 >= rows) continue;
+            if constexpr (C::F32) {
+#pragma unroll
+                for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        *reinterpret_cast<float4 *>(parts + r * C::PITCH + i * 32 + k * 16 + 2 * c2) =
+                            make_float4(o[4 * i][e * 2 + k], o[4 * i + 1][e * 2 + k], o[4 * i + 2][e * 2 + k], o[4 * i + 3][e * 2 + k]);
+            } else
 #pragma unroll
                 for (int i = 0; i < DP / 8; ++i) *reinterpret_cast<float2 *>(parts + r * C::PITCH + i * 8 + c2) = make_float2(o[i][e * 2], o[i][e * 2 + 1]);
         }
@@ -257,7 +350,8 @@ attention_rows_kernel(const __grid_constant__ RowsArgs t)
         }
         if (t.splits == 1) {
             const float inv = total == 0.f ? 0.f : 1.f / total;
-            *reinterpret_cast<uint2 *>((__nv_bfloat16 *)a.y + q_at(r, a.yp) + c) = make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
+            if constexpr (C::F32) *reinterpret_cast<float4 *>((float *)a.y + q_at(r, a.yp) + c) = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+            else *reinterpret_cast<uint2 *>((__nv_bfloat16 *)a.y + q_at(r, a.yp) + c) = make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
         } else {
             *reinterpret_cast<float4 *>(whole + r * C::PITCH + c) = x;
             if (c == 0) { sh->all_top[r] = most; sh->all_sum[r] = total; }
@@ -267,8 +361,8 @@ attention_rows_kernel(const __grid_constant__ RowsArgs t)
         __syncwarp();
         cluster_sync_all();
         if (!*abort_flag)
-            join_rows<__nv_bfloat16>(smem_u32(whole), C::PITCH, smem_u32(sh->all_top), smem_u32(sh->all_sum), rows, a.d, rank, t.splits, tid, R_THREADS,
-                                     [&](int r) { return (__nv_bfloat16 *)a.y + q_at(r, a.yp); });
+            join_rows<T>(smem_u32(whole), C::PITCH, smem_u32(sh->all_top), smem_u32(sh->all_sum), rows, a.d, rank, t.splits, tid, R_THREADS,
+                                     [&](int r) { return (T *)a.y + q_at(r, a.yp); });
         __syncwarp();
         cluster_sync_all();
     }
@@ -279,24 +373,31 @@ attention_rows_kernel(const __grid_constant__ RowsArgs t)
 }
 
 typedef void (*RowsKernel)(RowsArgs);
+struct RowsVariant {
+    RowsKernel kernel;
+    size_t bytes;
+};
+template <typename T, int DP> RowsVariant rows_variant() { return {attention_rows_kernel<T, DP>, RowsCfg<T, DP>::BYTES + sizeof(RowsShared)}; }
 
 }  // namespace
 
-bool attention_rows_covers(const AttnArgs &a, int dtype)
+bool attention_rows_covers(const AttnArgs &a)
 {
-    return dtype == DNB_BF16 && a.d <= 128 && (long long)a.lq * a.group <= 16 && (long long)a.n * a.kv_heads < 1LL << 28;
+    return a.d <= 128 && (long long)a.lq * a.group <= 16 && (long long)a.n * a.kv_heads < 1LL << 28;
 }
 
-int launch_attention_rows(const AttnArgs &a, cudaStream_t stream)
+int launch_attention_rows(const AttnArgs &a, int dtype, cudaStream_t stream)
 {
+    const bool f32 = dtype == DNB_F32, big = a.d > 64;
+    const uint64_t es = f32 ? 4 : 2;
     RowsArgs t;
     t.a = a;
     t.scale_log2 = a.scale * 1.4426950408889634f;
     auto map = [&](CUtensorMap *m, const void *data, int pitch) {
         const uint64_t dims[4] = {(uint64_t)a.d, (uint64_t)a.kv_heads, (uint64_t)a.lk, (uint64_t)a.kn};
-        const uint64_t strides[3] = {(uint64_t)a.d * 2, (uint64_t)pitch * 2, (uint64_t)a.lk * pitch * 2};
-        const uint32_t box[4] = {64, 1, R_KEYS, 1};
-        return encode_tensor_map(m, 1, 4, const_cast<void *>(data), dims, strides, box, 128);
+        const uint64_t strides[3] = {a.d * es, pitch * es, (uint64_t)a.lk * pitch * es};
+        const uint32_t box[4] = {f32 ? 32u : 64u, 1, R_KEYS, 1};
+        return encode_tensor_map(m, f32 ? 0 : 1, 4, const_cast<void *>(data), dims, strides, box, 128);
     };
     DNB_TRY(map(&t.tmk, a.k, a.kp));
     DNB_TRY(map(&t.tmv, a.v, a.vp));
@@ -305,17 +406,16 @@ int launch_attention_rows(const AttnArgs &a, cudaStream_t stream)
     const long long jobs = (long long)a.n * a.kv_heads;
     const int key_tiles = (a.lk + R_KEYS - 1) / R_KEYS;
     t.splits = 1;
-    while (t.splits < 8 && jobs * t.splits * 2 <= 2 * sm_count() && key_tiles >= t.splits * 8) t.splits *= 2;
-    const bool big = a.d > 64;
-    const RowsKernel kern = big ? attention_rows_kernel<128> : attention_rows_kernel<64>;
-    const size_t bytes = (big ? RowsCfg<128>::WORK : RowsCfg<64>::WORK) + sizeof(RowsShared);
-    static std::atomic<bool> done[64][2];
+    while (t.splits < 8 && jobs * t.splits * 2 <= 2 * sm_count() && key_tiles >= t.splits * (f32 ? 4 : 8)) t.splits *= 2;
+    const RowsVariant kern = f32 ? (big ? rows_variant<float, 128>() : rows_variant<float, 64>())
+                                 : (big ? rows_variant<__nv_bfloat16, 128>() : rows_variant<__nv_bfloat16, 64>());
+    static std::atomic<bool> done[64][4];
     int dev = 0;
     DNB_CUDA(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64) DNB_FAIL(DNB_ECUDA, "attention: device %d", dev);
-    if (!done[dev][big].load(std::memory_order_acquire)) {
-        DNB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-        done[dev][big].store(true, std::memory_order_release);
+    if (!done[dev][2 * f32 + big].load(std::memory_order_acquire)) {
+        DNB_CUDA(cudaFuncSetAttribute(kern.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kern.bytes));
+        done[dev][2 * f32 + big].store(true, std::memory_order_release);
     }
     cudaLaunchAttribute attrs[2];
     attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -325,11 +425,11 @@ int launch_attention_rows(const AttnArgs &a, cudaStream_t stream)
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(jobs * t.splits));
     cfg.blockDim = dim3(R_THREADS);
-    cfg.dynamicSmemBytes = bytes;
+    cfg.dynamicSmemBytes = kern.bytes;
     cfg.stream = stream;
     cfg.attrs = attrs;
     cfg.numAttrs = 2;
-    DNB_CUDA(cudaLaunchKernelEx(&cfg, kern, t));
+    DNB_CUDA(cudaLaunchKernelEx(&cfg, kern.kernel, t));
     DNB_LAUNCH_CHECK("attention");
     return DNB_OK;
 }
