@@ -85,43 +85,51 @@ __device__ __forceinline__ void share_of_keys(int keys, int size, int rank, int 
 
 // Joins the rows that the CTAs of a cluster hold of the same queries: in every CTA, at the same addresses of shared memory, row r's sum of weighted
 // values at rows + r * pitch floats, its largest scaled score (log2) in tops[r] and its sum of weights in sums[r] (0: its row holds nothing).
-// Eight channels an item, the items dealt out over the cluster's threads; the additions in the order of the ranks, which is the keys'.
+// Four channels an item, the items dealt out over the cluster's threads; the additions in the order of the ranks, which is the keys'.  All of an item's
+// loads are on their way before the first is used: one trip to the neighbours, not one a neighbour.  N: the CTAs, rounded up to 2, 4 or 8.
 // out(r): where row r's d channels go, or null.
+template <typename T, int N, typename Out>
+__device__ __forceinline__ void join_rows_of(uint32_t rows, int pitch, uint32_t tops, uint32_t sums, int count, int d, int rank, int splits, int tid, int threads, Out out)
+{
+    const int chunks = d / 4;
+    for (int i = tid * splits + rank; i < count * chunks; i += threads * splits) {
+        const int r = i / chunks, c = (i - r * chunks) * 4;
+        T *to = out(r);
+        if (!to) continue;
+        float top[N], weight[N];
+        float4 x[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const uint32_t from = k < splits ? k : 0;
+            top[k] = ld_peer1(tops + 4 * r, from);
+            weight[k] = ld_peer1(sums + 4 * r, from);
+            x[k] = ld_peer(rows + (r * pitch + c) * 4, from);
+        }
+        float most = -INFINITY, total = 0.f;
+#pragma unroll
+        for (int k = 0; k < N; ++k) most = fmaxf(most, top[k]);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const bool has = k < splits && weight[k] != 0.f;
+            const float w = top[k] == most ? 1.f : ex2(top[k] - most);
+            total = has ? fmaf(weight[k], w, total) : total;
+            o.x = has ? fmaf(x[k].x, w, o.x) : o.x;
+            o.y = has ? fmaf(x[k].y, w, o.y) : o.y;
+            o.z = has ? fmaf(x[k].z, w, o.z) : o.z;
+            o.w = has ? fmaf(x[k].w, w, o.w) : o.w;
+        }
+        const float inv = total == 0.f ? 0.f : 1.f / total;
+        if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2 *>(to + c) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+        else *reinterpret_cast<float4 *>(to + c) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    }
+}
 template <typename T, typename Out>
 __device__ __forceinline__ void join_rows(uint32_t rows, int pitch, uint32_t tops, uint32_t sums, int count, int d, int rank, int splits, int tid, int threads, Out out)
 {
-    const int chunks = d / 8;
-    for (int i = tid * splits + rank; i < count * chunks; i += threads * splits) {
-        const int r = i / chunks, c = (i - r * chunks) * 8;
-        T *to = out(r);
-        if (!to) continue;
-        float most = -INFINITY, top[8], weight[8], total = 0.f;
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (k < splits) {
-                top[k] = ld_peer1(tops + 4 * r, k);
-                weight[k] = ld_peer1(sums + 4 * r, k);
-                most = fmaxf(most, top[k]);
-            }
-        float o[8] = {};
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (k < splits && weight[k] != 0.f) {
-                const float w = top[k] == most ? 1.f : ex2(top[k] - most);
-                total += weight[k] * w;
-                const float4 x = ld_peer(rows + (r * pitch + c) * 4, k), z = ld_peer(rows + (r * pitch + c + 4) * 4, k);
-                o[0] = fmaf(x.x, w, o[0]); o[1] = fmaf(x.y, w, o[1]); o[2] = fmaf(x.z, w, o[2]); o[3] = fmaf(x.w, w, o[3]);
-                o[4] = fmaf(z.x, w, o[4]); o[5] = fmaf(z.y, w, o[5]); o[6] = fmaf(z.z, w, o[6]); o[7] = fmaf(z.w, w, o[7]);
-            }
-        const float inv = total == 0.f ? 0.f : 1.f / total;
-        if constexpr (sizeof(T) == 2) {
-            *reinterpret_cast<uint4 *>(to + c) = make_uint4(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv), pack_bf16(o[4] * inv, o[5] * inv),
-                                                            pack_bf16(o[6] * inv, o[7] * inv));
-        } else {
-            *reinterpret_cast<float4 *>(to + c) = make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-            *reinterpret_cast<float4 *>(to + c + 4) = make_float4(o[4] * inv, o[5] * inv, o[6] * inv, o[7] * inv);
-        }
-    }
+    if (splits <= 2) join_rows_of<T, 2>(rows, pitch, tops, sums, count, d, rank, splits, tid, threads, out);
+    else if (splits <= 4) join_rows_of<T, 4>(rows, pitch, tops, sums, count, d, rank, splits, tid, threads, out);
+    else join_rows_of<T, 8>(rows, pitch, tops, sums, count, d, rank, splits, tid, threads, out);
 }
 
 }  // namespace dnb

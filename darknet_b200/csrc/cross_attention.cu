@@ -5,6 +5,7 @@
 // A query that may see no key gets zeros.
 #include <math.h>
 
+#include <atomic>
 #include <new>
 
 #include "attention.h"
@@ -85,6 +86,47 @@ int launch_attention_simple(const AttnArgs &a, int dtype, cudaStream_t s)
     if (dtype == DNB_BF16) DNB_CUDA(launch_overlapped(attention_simple_kernel<__nv_bfloat16>, dim3((unsigned)blocks), 128, 0, s, a));
     else DNB_CUDA(launch_overlapped(attention_simple_kernel<float>, dim3((unsigned)blocks), 128, 0, s, a));
     DNB_LAUNCH_CHECK("attention");
+    return DNB_OK;
+}
+
+int split_keys(long long jobs, int key_tiles, const int room[4], double start, double join)
+{
+    int best = 1;
+    double least = 0.0;
+    for (int i = 0, s = 1; i < 4 && (s == 1 || s <= key_tiles); ++i, s *= 2) {
+        if (room[i] < s) continue;
+        const double waves = (double)((jobs * s + room[i] - 1) / room[i]), cost = waves * ((key_tiles + s - 1) / s + start + (s > 1 ? join * s : 0.0));
+        if (s == 1 || cost < least) {
+            best = s;
+            least = cost;
+        }
+    }
+    return best;
+}
+
+int cluster_room(const void *kernel, int slot, int threads, size_t smem, int room[4])
+{
+    static std::atomic<int> known[64][8][4];
+    int dev = 0;
+    DNB_CUDA(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64) DNB_FAIL(DNB_ECUDA, "attention: device %d", dev);
+    for (int i = 0; i < 4; ++i) {
+        room[i] = known[dev][slot][i].load(std::memory_order_relaxed);
+        if (room[i]) continue;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = 1u << i; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(1u << i);
+        cfg.blockDim = dim3((unsigned)threads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        int clusters = 0;
+        DNB_CUDA(cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg));
+        room[i] = clusters > 0 ? clusters << i : i == 0 ? sm_count() : -1;
+        known[dev][slot][i].store(room[i], std::memory_order_relaxed);
+    }
     return DNB_OK;
 }
 

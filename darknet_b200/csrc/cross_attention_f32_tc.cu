@@ -24,6 +24,7 @@ namespace {
 constexpr int KEYS = 64, SOFT = 8, CONVERT = 8, MMA_WARP = SOFT + CONVERT, THREADS = 640;
 // Registers: 640 threads start with 96 each; 256 * 144 + 384 * 64 = 640 * 96.
 constexpr int SOFT_REGS = 144, OTHER_REGS = 64;
+constexpr int PASSES = 2;
 constexpr uint32_t Q_BOX = 128 * 128, KV_BOX = KEYS * 128;   // 64 channels of a part: of the queries, of a tile's keys or values
 
 struct F32TcShared {
@@ -169,36 +170,42 @@ attention_f32_tc_kernel(const __grid_constant__ F32TcArgs t)
             const int pitch = is_v ? a.vp : a.kp;
             const float *src = (const float *)(is_v ? a.v : a.k) + (size_t)(a.kn == 1 ? 0 : image) * a.lk * pitch + kv_head * a.d;
             uint64_t *full = is_v ? sh->v_full : sh->k_full, *free_ = is_v ? sh->v_free : sh->k_free;
+            // A pass: 2^turn lanes a row, eight channels each, a box's channels; PASSES of them are on their way while as many are split.
+            const int turn = a.d > 32 ? 3 : a.d > 16 ? 2 : 1, c0 = wt & ((1 << turn) - 1), row0 = wt >> turn, pass_rows = CONVERT / 2 * 32 >> turn;
+            const int per_box = (KEYS + PASSES * pass_rows - 1) / (PASSES * pass_rows), per_tile = per_box * ((a.d + 63) >> 6);
+            struct Batch {
+                float4 x[PASSES], y[PASSES];
+            };
+            auto load = [&](Batch &b, int j, int at) {
+                const int c = (at >= per_box ? 8 : 0) + c0, base = (at >= per_box ? at - per_box : at) * PASSES * pass_rows + row0;
+#pragma unroll
+                for (int k = 0; k < PASSES; ++k) {
+                    const int r = base + k * pass_rows, key = (first + j) * KEYS + r;
+                    b.x[k] = b.y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    // zeros where there is no key, or none that any query sees
+                    if (r < KEYS && key < keys && 8 * c < a.d && !(mask && !mask[key])) {
+                        const float4 *p = reinterpret_cast<const float4 *>(src + (size_t)key * pitch + 8 * c);
+                        b.x[k] = __ldg(p);
+                        b.y[k] = __ldg(p + 1);
+                    }
+                }
+            };
             int stage = 0;
             uint32_t phase = 0;
+            Batch next;
+            if (tiles > 0) load(next, 0, 0);
             for (int j = 0; j < tiles; ++j) {
-                const int key0 = (first + j) * KEYS;
                 uint8_t *to = smem_raw + (is_v ? C::V_AT : C::K_AT) + stage * 3 * C::KV_PART;
-                bool waited = false;
-                for (int i0 = wt; i0 < KEYS * chunks; i0 += 2 * CONVERT / 2 * 32) {
-                    float4 x[2], y[2];
-                    int r[2], c[2];
+#pragma unroll 1
+                for (int at = 0; at < per_tile; ++at) {
+                    const Batch b = next;
+                    const bool last = at + 1 == per_tile;
+                    if (!last || j + 1 < tiles) load(next, last ? j + 1 : j, last ? 0 : at + 1);
+                    if (at == 0) mbar_wait_tight(smem_u32(&free_[stage]), phase ^ 1, abort_flag, a.status, AT_SLOT, a.polls);
+                    const int c = (at >= per_box ? 8 : 0) + c0, base = (at >= per_box ? at - per_box : at) * PASSES * pass_rows + row0;
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const int i = i0 + k * CONVERT / 2 * 32;
-                        r[k] = i / chunks;
-                        c[k] = i - r[k] * chunks;
-                        x[k] = y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                        const int key = key0 + r[k];
-                        // zeros where there is no key, or none that any query sees
-                        if (i < KEYS * chunks && key < keys && 8 * c[k] < a.d && !(mask && !mask[key])) {
-                            const float4 *p = reinterpret_cast<const float4 *>(src + (size_t)key * pitch + 8 * c[k]);
-                            x[k] = __ldg(p);
-                            y[k] = __ldg(p + 1);
-                        }
-                    }
-                    if (!waited) {                                      // with the first loads on their way
-                        waited = true;
-                        mbar_wait_tight(smem_u32(&free_[stage]), phase ^ 1, abort_flag, a.status, AT_SLOT, a.polls);
-                    }
-#pragma unroll
-                    for (int k = 0; k < 2; ++k)
-                        if (i0 + k * CONVERT / 2 * 32 < KEYS * chunks) store_parts(to, KV_BOX, C::KV_PART, r[k], c[k], x[k], y[k]);
+                    for (int k = 0; k < PASSES; ++k)
+                        if (base + k * pass_rows < KEYS && c < chunks) store_parts(to, KV_BOX, C::KV_PART, base + k * pass_rows, c, b.x[k], b.y[k]);
                 }
                 fence_async_smem();
                 __syncwarp();
@@ -434,11 +441,14 @@ int launch_attention_f32_tc(const AttnArgs &a, cudaStream_t stream)
         DNB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, conv_tc_max_smem()));
         done[dev][which].store(true, std::memory_order_release);
     }
-    // Fewer CTAs than SMs: split the keys, two tiles of them a CTA at least.
     const long long jobs = (long long)a.n * a.kv_heads * t.q_tiles;
     const int key_tiles = (a.lk + KEYS - 1) / KEYS;
-    t.splits = 1;
-    while (t.splits < 8 && jobs * t.splits * 2 <= sm_count() && key_tiles >= t.splits * 4) t.splits *= 2;
+    const size_t bytes = tmem_smem(a.d > 64 ? F32TcCfg<128>::BYTES : F32TcCfg<64>::BYTES, 512);
+    // Heads of 64, us over 1 / 2 / 4 / 8 CTAs a job: 8 jobs of 6 tiles 17.6 / 14.3 / 12.6 / 15.1, 32 jobs of 23 49.0 / 31.5 / 21.6 / 51.6, 200 jobs of 91
+    // 360 / 295 / 380.  A tile's time is 1.9 us (4.6 of heads of 128).
+    int room[4];
+    DNB_TRY(cluster_room((const void *)kern, 4 + which, THREADS, bytes, room));
+    t.splits = split_keys(jobs, key_tiles, room, 3.0, 0.5);
     cudaLaunchAttribute attrs[2];
     attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attrs[0].val.programmaticStreamSerializationAllowed = pdl_enabled() && jobs * t.splits <= EARLY_BLOCKS ? 1 : 0;
@@ -447,7 +457,7 @@ int launch_attention_f32_tc(const AttnArgs &a, cudaStream_t stream)
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(jobs * t.splits));
     cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = tmem_smem(a.d > 64 ? F32TcCfg<128>::BYTES : F32TcCfg<64>::BYTES, 512);
+    cfg.dynamicSmemBytes = bytes;
     cfg.stream = stream;
     cfg.attrs = attrs;
     cfg.numAttrs = 2;

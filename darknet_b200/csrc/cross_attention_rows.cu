@@ -401,12 +401,13 @@ int launch_attention_rows(const AttnArgs &a, int dtype, cudaStream_t stream)
     };
     DNB_TRY(map(&t.tmk, a.k, a.kp));
     DNB_TRY(map(&t.tmv, a.v, a.vp));
-    // Two blocks an SM: split the keys while there is room for twice the blocks, four tiles a block at least (a ring is
-    // on its way at once; joining costs a microsecond: one token, 8 heads of 64, 361 keys 6.8 us over four blocks a head, 6.3 over one).
+    // Two blocks an SM: the keys over as many of them as there is room for.  One token, us over 1 / 2 / 4 / 8 blocks a head: 8 heads of 64, 361 keys
+    // 6.6 / 6.1 / 6.1 / 5.8 (f32 11.0 / 8.0 / 7.0 / 5.7), 1444 keys 14.7 / 10.6 / 7.6 / 6.6; 80 heads over 1 / 2 / 3 / 4 15.1 / 11.3 / 9.7 / 16.0.
     const long long jobs = (long long)a.n * a.kv_heads;
     const int key_tiles = (a.lk + R_KEYS - 1) / R_KEYS;
-    t.splits = 1;
-    while (t.splits < 8 && jobs * t.splits * 2 <= 2 * sm_count() && key_tiles >= t.splits * (f32 ? 4 : 8)) t.splits *= 2;
+    const long long room = 2LL * sm_count() / jobs;
+    t.splits = room < 2 ? 1 : (int)(room < 8 ? room : 8);
+    if (t.splits > key_tiles) t.splits = key_tiles;
     const RowsVariant kern = f32 ? (big ? rows_variant<float, 128>() : rows_variant<float, 64>())
                                  : (big ? rows_variant<__nv_bfloat16, 128>() : rows_variant<__nv_bfloat16, 64>());
     static std::atomic<bool> done[64][4];

@@ -566,14 +566,17 @@ int launch_attention_tc(const AttnArgs &a, cudaStream_t stream)
     DNB_TRY(map(&t.tmq, a.q, a.heads, a.qp, a.lq, a.n, a.group, t.q_tokens));
     DNB_TRY(map(&t.tmk, a.k, a.kv_heads, a.kp, a.lk, a.kn, 1, 128));
     DNB_TRY(map(&t.tmv, a.v, a.kv_heads, a.vp, a.lk, a.kn, 1, 128));
-    // Fewer CTAs than SMs: split the keys, two tiles of them a CTA at least.
     const long long jobs = (long long)a.n * a.kv_heads * t.q_tiles;
     const int key_tiles = (a.lk + 127) / 128;
-    t.splits = 1;
-    while (t.splits < 8 && jobs * t.splits * 2 <= sm_count() && key_tiles >= t.splits * 4) t.splits *= 2;
     const int which = (a.d > 64 ? 2 : 0) + (a.mask ? 1 : 0);
     const Kernel kern = which == 0 ? attention_tc_kernel<64, false> : which == 1 ? attention_tc_kernel<64, true> : which == 2 ? attention_tc_kernel<128, false> : attention_tc_kernel<128, true>;
     DNB_TRY(prepare(kern, which));
+    const size_t bytes = tmem_smem(a.d > 64 ? Cfg<128>::BYTES : Cfg<64>::BYTES, 512);
+    // Heads of 64, us over 1 / 2 / 4 / 8 CTAs a job: 8 jobs of 3 tiles 9.5 / 11.4 / 13.5, of 12 22.8 / 17.0 / 15.1 / 19.3, of 46 69.7 / 41.2 / 27.8 / 25.4;
+    // 152 jobs of 46 144 / 128 / 145, 384 jobs of 46 216 / 249.  A tile's time is 1.4 us (1.8 of heads of 128).
+    int room[4];
+    DNB_TRY(cluster_room((const void *)kern, which, THREADS, bytes, room));
+    t.splits = a.mask ? split_keys(jobs, key_tiles, room, 1.5, 0.4) : split_keys(jobs, key_tiles, room, 4.0, 1.0);   // a masked tile takes 2.7 times as long
     cudaLaunchAttribute attrs[2];
     attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attrs[0].val.programmaticStreamSerializationAllowed = pdl_enabled() && jobs * t.splits <= EARLY_BLOCKS ? 1 : 0;
@@ -582,7 +585,7 @@ int launch_attention_tc(const AttnArgs &a, cudaStream_t stream)
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(jobs * t.splits));
     cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = tmem_smem(a.d > 64 ? Cfg<128>::BYTES : Cfg<64>::BYTES, 512);
+    cfg.dynamicSmemBytes = bytes;
     cfg.stream = stream;
     cfg.attrs = attrs;
     cfg.numAttrs = 2;
