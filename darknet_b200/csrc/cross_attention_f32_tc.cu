@@ -27,7 +27,7 @@ constexpr int SOFT_REGS = 144, OTHER_REGS = 64;
 constexpr int PASSES = 2;
 constexpr uint32_t Q_BOX = 128 * 128, KV_BOX = KEYS * 128;   // 64 channels of a part: of the queries, of a tile's keys or values
 
-struct F32TcShared {
+struct alignas(16) F32TcShared {
     uint64_t q_full, k_full[2], k_free[2], v_full[2], v_free[2], s_full[2], s_read[2], p_full[2], o_full, o_read, met[4];
     uint32_t tmem_base;
     int abort_flag;
@@ -40,11 +40,11 @@ struct F32TcArgs {
     float scale_log2;
 };
 
-template <int DP> struct F32TcCfg {
+template <int DP, bool MASK> struct F32TcCfg {
     static constexpr int BOXES = DP / 64, STAGES = DP == 64 ? 2 : 1, PITCH = DP + 4;
     static constexpr uint32_t Q_PART = BOXES * Q_BOX, KV_PART = BOXES * KV_BOX;
     static constexpr uint32_t K_AT = 3 * Q_PART, V_AT = K_AT + STAGES * 3 * KV_PART, WORK = V_AT + STAGES * 3 * KV_PART;
-    static constexpr uint32_t BYTES = WORK + sizeof(F32TcShared);
+    static constexpr uint32_t MASKS_AT = WORK + sizeof(F32TcShared), BYTES = MASKS_AT + (MASK ? SOFT * MaskRows<32>::BYTES : 0);
     static constexpr uint32_t S_COL = 0, P_COL = 128, O_COL = 320;       // two of 64, two of 3 * 32, one of DP
     static_assert(130 * PITCH * 4 <= (int)WORK && BYTES <= 232448, "fits an SM");
 };
@@ -83,7 +83,7 @@ template <int DP, bool MASK>
 __global__ void __launch_bounds__(THREADS, 1)
 attention_f32_tc_kernel(const __grid_constant__ F32TcArgs t)
 {
-    using C = F32TcCfg<DP>;
+    using C = F32TcCfg<DP, MASK>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const AttnArgs &a = t.a;
     const uint32_t smem = smem_u32(smem_raw);
@@ -292,7 +292,11 @@ attention_f32_tc_kernel(const __grid_constant__ F32TcArgs t)
     const int token = token0 + row / a.group;
     const uint32_t met = smem_u32(&sh->met[warp & 3]);
     const uint8_t *mask = nullptr;
-    if (MASK) mask = a.mask + (long long)image * a.mask_image + (long long)(valid ? token : a.lq - 1) * a.mask_query;
+    const uint32_t mask_at = smem + C::MASKS_AT + warp * MaskRows<32>::BYTES;
+    if (MASK) {
+        mask = a.mask + (long long)image * a.mask_image + (long long)(valid ? token : a.lq - 1) * a.mask_query;
+        if (tiles > 0) mask_fetch<32>(mask_at, mask, first * KEYS + half * 32, keys, lane);
+    }
     float o[DP / 2] = {}, top = -INFINITY, sum = 0.f;
     // adds the tile before, which was weighed against the same maximum as o
     auto add_tile = [&](int j, float shrink) {
@@ -315,21 +319,8 @@ attention_f32_tc_kernel(const __grid_constant__ F32TcArgs t)
         const int key0 = (first + j) * KEYS + half * 32, left = keys - key0;
         uint32_t bits = left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1u : 0u;
         if (MASK) {
-            // The rows' masks, 32 keys of a row a load, sixteen rows' loads in flight together; one row's where all are alike.
-            const int rows = a.mask_query == 0 ? 1 : 32;
-            for (int i0 = 0; i0 < rows; i0 += 16) {
-                uint8_t m[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const uint8_t *p = reinterpret_cast<const uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mask), i0 + i)) + key0;
-                    m[i] = i0 + i < rows && lane < left ? p[lane] : 0;
-                }
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const uint32_t now = __ballot_sync(0xffffffffu, m[i] != 0);
-                    if (rows == 1 ? i == 0 : lane == i0 + i) bits = now;
-                }
-            }
+            mask_bits<32>(mask_at, mask, key0, lane, &bits);
+            if (j + 1 < tiles) mask_fetch<32>(mask_at, mask, key0 + KEYS, keys, lane);
         }
         mbar_wait_tight(smem_u32(&sh->s_full[j & 1]), j >> 1 & 1, abort_flag, a.status, AT_SCORES, a.polls);
         tc_fence_after();
@@ -443,7 +434,7 @@ int launch_attention_f32_tc(const AttnArgs &a, cudaStream_t stream)
     }
     const long long jobs = (long long)a.n * a.kv_heads * t.q_tiles;
     const int key_tiles = (a.lk + KEYS - 1) / KEYS;
-    const size_t bytes = tmem_smem(a.d > 64 ? F32TcCfg<128>::BYTES : F32TcCfg<64>::BYTES, 512);
+    const size_t bytes = tmem_smem(a.mask ? (a.d > 64 ? F32TcCfg<128, true>::BYTES : F32TcCfg<64, true>::BYTES) : a.d > 64 ? F32TcCfg<128, false>::BYTES : F32TcCfg<64, false>::BYTES, 512);
     // Heads of 64, us over 1 / 2 / 4 / 8 CTAs a job: 8 jobs of 6 tiles 17.6 / 14.3 / 12.6 / 15.1, 32 jobs of 23 49.0 / 31.5 / 21.6 / 51.6, 200 jobs of 91
     // 360 / 295 / 380.  A tile's time is 1.9 us (4.6 of heads of 128).
     int room[4];

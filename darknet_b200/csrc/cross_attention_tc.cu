@@ -33,7 +33,7 @@ constexpr int MAX_STAGES = 12;
 constexpr uint32_t BOX_BYTES = 128 * 128;         // 64 channels of 128 rows
 constexpr float MOVE = 8.f;                       // how far (log2) scores may outgrow the running maximum
 
-struct Shared {
+struct alignas(16) Shared {
     uint64_t q_full, full[MAX_STAGES], empty[MAX_STAGES], s_full[2], s_read[2], p_full[2], o_full[2], met[8];
     uint32_t tmem_base;
     int abort_flag;
@@ -88,10 +88,10 @@ __device__ __forceinline__ uint64_t desc_values(uint32_t addr)
     return d;
 }
 // DP: channels of a head as they lie in shared memory, 64 or 128 (TMA fills what the head does not have with zeros).
-template <int DP> struct Cfg {
+template <int DP, bool MASK> struct Cfg {
     static constexpr int BOXES = DP / 64;
     static constexpr uint32_t TILE_BYTES = BOXES * BOX_BYTES;
-    static constexpr int STAGES = DP == 128 ? 5 : 11;
+    static constexpr int STAGES = DP == 128 ? (MASK ? 3 : 5) : MASK ? 9 : 11;
     static constexpr uint32_t WORK = 2 * TILE_BYTES + STAGES * TILE_BYTES;
     static constexpr int PITCH = DP + 4;          // of a row of sums, for the join
     // TMEM: the scores of both tiles, their outputs and, where there is room, weights of their own.  Then the next tile's scores are made while the
@@ -100,7 +100,7 @@ template <int DP> struct Cfg {
     static constexpr uint32_t O_AT = 256, P_AT = OWN_P ? 256 + 2 * DP : 0, P_STEP = OWN_P ? 64 : 128;
     // The halves' largest scores: one set for each of two tiles of keys where the next scores may be there before this tile's have been compared.
     static constexpr int SETS = OWN_P ? 2 : 1;
-    static constexpr uint32_t BYTES = WORK + sizeof(Shared) + SETS * 2048;
+    static constexpr uint32_t MASKS_AT = WORK + sizeof(Shared) + SETS * 2048, BYTES = MASKS_AT + (MASK ? SOFT_WARPS * MaskRows<64>::BYTES : 0);
     static_assert(258 * PITCH * 4 + 2048 <= WORK && STAGES <= MAX_STAGES, "the rows' sums fit where the operands were");
     static_assert(BYTES <= 232448, "fits an SM");
 };
@@ -109,7 +109,7 @@ template <int DP, bool MASK>
 __global__ void __launch_bounds__(THREADS, 1)
 attention_tc_kernel(const __grid_constant__ TcAttnArgs t)
 {
-    using C = Cfg<DP>;
+    using C = Cfg<DP, MASK>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const AttnArgs &a = t.a;
     const uint32_t smem = smem_u32(smem_raw);
@@ -337,31 +337,21 @@ attention_tc_kernel(const __grid_constant__ TcAttnArgs t)
         const float scale = t.scale_log2;
         const uint32_t met = smem_u32(&sh->met[s * 4 + (warp & 3)]);    // this warp and the one with the rows' other half
         const uint8_t *mask = nullptr;
-        if (MASK) mask = a.mask + (long long)image * a.mask_image + (valid ? r_token : a.lq - 1) * a.mask_query;
+        const uint32_t mask_at = smem + C::MASKS_AT + warp * MaskRows<64>::BYTES;
+        if (MASK) {
+            mask = a.mask + (long long)image * a.mask_image + (valid ? r_token : a.lq - 1) * a.mask_query;
+            if (tiles > 0) mask_fetch<64>(mask_at, mask, t0 * 128 + half * 64, keys, lane);
+        }
         int stage = 1;
         uint32_t phase = 0;                                             // of V's slots
         for (int j = 0; j < tiles; ++j) {
             const int key0 = (t0 + j) * 128, left = keys - key0, col0 = half * 64;
             uint32_t bits[2] = {0xffffffffu, 0xffffffffu};
+            uint8_t seen = 1;                                           // with one mask for all queries: key `row` of the tile
             if (MASK) {
-                // The rows' masks, 32 keys of a row a load, sixteen rows' loads in flight together; one row's where all are alike.
-                const int rows = a.mask_query == 0 ? 1 : 32;
-                for (int i0 = 0; i0 < rows; i0 += 16) {
-                    uint8_t m[16][2];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const uint8_t *p = reinterpret_cast<const uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mask), i0 + i)) + key0 + col0;
-#pragma unroll
-                        for (int w = 0; w < 2; ++w) m[i][w] = i0 + i < rows && col0 + lane + 32 * w < left ? p[lane + 32 * w] : 0;
-                    }
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-#pragma unroll
-                        for (int w = 0; w < 2; ++w) {
-                            const uint32_t now = __ballot_sync(0xffffffffu, m[i][w] != 0);
-                            if (rows == 1 ? i == 0 : lane == i0 + i) bits[w] = now;
-                        }
-                }
+                mask_bits<64>(mask_at, mask, key0 + col0, lane, bits);
+                if (j + 1 < tiles) mask_fetch<64>(mask_at, mask, key0 + 128 + col0, keys, lane);
+                if (a.mask_query == 0 && row < left) seen = mask[key0 + row];
             } else if (left < 128) {
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
@@ -444,9 +434,7 @@ attention_tc_kernel(const __grid_constant__ TcAttnArgs t)
             // Values that no weight reaches may be anything, and zero times infinity is no number: zeros in their place.  (Both tiles write them.)
             if ((left < 128 && keys < a.lk) || (MASK && a.mask_query == 0)) {
                 mbar_wait_tight(smem_u32(&sh->full[stage]), phase, abort_flag, a.status, AT_VALUES, a.polls);
-                bool hidden = row >= left;
-                if (MASK && a.mask_query == 0 && !hidden) hidden = mask[key0 + row] == 0;
-                if (hidden) {
+                if (row >= left || (MASK && !seen)) {
                     const uint32_t at = 2 * C::TILE_BYTES + stage * C::TILE_BYTES + row * 128;
 #pragma unroll
                     for (int b = half; b < C::BOXES; b += 2)
@@ -571,12 +559,12 @@ int launch_attention_tc(const AttnArgs &a, cudaStream_t stream)
     const int which = (a.d > 64 ? 2 : 0) + (a.mask ? 1 : 0);
     const Kernel kern = which == 0 ? attention_tc_kernel<64, false> : which == 1 ? attention_tc_kernel<64, true> : which == 2 ? attention_tc_kernel<128, false> : attention_tc_kernel<128, true>;
     DNB_TRY(prepare(kern, which));
-    const size_t bytes = tmem_smem(a.d > 64 ? Cfg<128>::BYTES : Cfg<64>::BYTES, 512);
+    const size_t bytes = tmem_smem(a.mask ? (a.d > 64 ? Cfg<128, true>::BYTES : Cfg<64, true>::BYTES) : a.d > 64 ? Cfg<128, false>::BYTES : Cfg<64, false>::BYTES, 512);
     // Heads of 64, us over 1 / 2 / 4 / 8 CTAs a job: 8 jobs of 3 tiles 9.5 / 11.4 / 13.5, of 12 22.8 / 17.0 / 15.1 / 19.3, of 46 69.7 / 41.2 / 27.8 / 25.4;
     // 152 jobs of 46 144 / 128 / 145, 384 jobs of 46 216 / 249.  A tile's time is 1.4 us (1.8 of heads of 128).
     int room[4];
     DNB_TRY(cluster_room((const void *)kern, which, THREADS, bytes, room));
-    t.splits = a.mask ? split_keys(jobs, key_tiles, room, 1.5, 0.4) : split_keys(jobs, key_tiles, room, 4.0, 1.0);   // a masked tile takes 2.7 times as long
+    t.splits = a.mask ? split_keys(jobs, key_tiles, room, 2.5, 0.6) : split_keys(jobs, key_tiles, room, 4.0, 1.0);   // a masked tile takes 1.7 times as long
     cudaLaunchAttribute attrs[2];
     attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attrs[0].val.programmaticStreamSerializationAllowed = pdl_enabled() && jobs * t.splits <= EARLY_BLOCKS ? 1 : 0;
