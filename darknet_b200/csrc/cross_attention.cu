@@ -193,7 +193,7 @@ extern "C" int dnb_attention_forward(dnb_attention_plan *p, const dnb_tensor *q,
     if (k->n != q->n && k->n != 1) DNB_FAIL(DNB_EINVAL, "attention: keys of %d images for queries of %d (one for all, or one each)", k->n, q->n);
     for (const dnb_tensor *t : {q, k, v})
         if (t->data == y->data) DNB_FAIL(DNB_EINVAL, "attention: the output is an input's memory");
-    if ((long long)q->h * q->w >= 1LL << 31 || (long long)k->h * k->w >= 1LL << 31) DNB_FAIL(DNB_EUNSUPPORTED, "attention: more than 2^31 tokens an image");
+    if ((long long)q->h * q->w > 1LL << 30 || (long long)k->h * k->w > 1LL << 30) DNB_FAIL(DNB_EUNSUPPORTED, "attention: more than 2^30 tokens an image");
     AttnArgs a = {};
     a.q = q->data; a.k = k->data; a.v = v->data; a.y = y->data;
     a.n = q->n; a.kn = k->n;
