@@ -407,6 +407,10 @@ int launch_attention_rows(const AttnArgs &a, int dtype, cudaStream_t stream)
     const int key_tiles = (a.lk + R_KEYS - 1) / R_KEYS;
     const long long room = 2LL * sm_count() / jobs;
     t.splits = room < 2 ? 1 : (int)(room < 8 ? room : 8);
+    // f32 images of lengths of their own: twice the blocks while each keeps twelve tiles, so that a short image's place is taken by a long one's keys
+    // (32 tokens over maps of up to 5776, 4 key heads of 128: 127 us, from 145; bf16 46 either way).
+    if (f32 && a.lengths)
+        while (t.splits < 8 && (t.splits + 1) * jobs <= 4LL * sm_count() && key_tiles >= 12 * (t.splits + 1)) ++t.splits;
     if (t.splits > key_tiles) t.splits = key_tiles;
     const RowsVariant kern = f32 ? (big ? rows_variant<float, 128>() : rows_variant<float, 64>())
                                  : (big ? rows_variant<__nv_bfloat16, 128>() : rows_variant<__nv_bfloat16, 64>());
