@@ -8,7 +8,9 @@
 //
 // A CTA holds 128 query rows (a row: one query token of one head; heads that share keys lie side by side) and walks over the keys 64 at a time: eight warps make
 // the weights (half a row a thread) and add the tiles up, four split the keys into parts, four the values, one issues the products.  S and P have two places
-// each, so that a tile's scores are made while the tile before is weighed.  The tensor pipe bounds it: six times the bf16 kernel's products.
+// each, so that a tile's scores are made while the tile before is weighed.  A tile's chain of hand-overs bounds it, 1.9 us of 64 keys and heads of 64 (the
+// products alone would take 0.8), 4.6 of heads of 128, whose keys and values have one place each beside three parts of queries.
+// Measured: 8 x 100 queries over 1444 keys, 8 heads of 32, 25 us; 4 x 2000 over 5776, 8 heads of 64, 692 us (137 TFLOP/s of f32 products; 32 on the CUDA cores).
 // Few rows: the keys are split over the CTAs of a cluster, which join their sums through distributed shared memory.
 #include <atomic>
 

@@ -4,6 +4,7 @@
 // them an SM) on the way.  Four warps, 16 keys of a tile each, multiply them by up to 16 rows with mma.sync: the 128 rows of a tcgen05 product would be
 // empty but for a few, its TMEM round trip is a latency for each tile, and the arithmetic is far from any bound either way.  A warp has a running maximum
 // and sum of its own keys; warps, and the CTAs of a cluster that share the keys of one head, meet once at the end.
+// Measured: 32 tokens over 5776 keys, 16 heads over 4 of 128: 61 us in bf16 (6.2 TB/s), 153 in f32 (5.0 TB/s); one token over 361 keys, 8 heads of 64: 5.9 us back to back.
 //
 // f32 operands are sums of three bf16 numbers (24 bits of mantissa), their product the six products of parts that reach 2^-24 of it, smallest first; a tile's
 // sums are added to the rows' in fp32, since the tensor cores' sums lose a little at each addition.  A lane reads four channels of a key at once: which

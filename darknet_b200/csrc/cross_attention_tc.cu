@@ -6,6 +6,8 @@
 //   P = exp2(S * scale * log2 e - m)   eight warps a tile, half a row a thread, out of TMEM and back into it as bf16
 //   O += P V    tcgen05.mma, P from TMEM, V from shared memory as it lies (channels innermost: a transposed operand), O in TMEM (fp32)
 // While one tile's warps take exponentials, the tensor cores multiply the other tile's: the two are never both idle.
+// Measured: 8 x 5776 queries over 5776 keys, 8 heads of 128 916 us (1190 TFLOP/s, tensor pipe and exponentials 58 % each), of 64 710 us (770 TFLOP/s): there
+// the softmax's chain bounds it (exponentials for nothing would save 4 %; a share of them as polynomials on the FMA pipe costs 4 to 10 %).
 //
 // The running maximum m moves only when a row's largest score has outgrown it by more than 2^8 (every weight is then at most 256 times what
 // the largest should be, far inside bf16's and fp32's range); until then O needs no correction.  The sum of the weights is kept in fp32 of the

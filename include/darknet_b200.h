@@ -273,6 +273,9 @@ int dnb_softmax_forward(const dnb_tensor *x, const dnb_tensor *y, int groups, fl
  * one dtype (f32 or bf16); a token is a pixel, n * h * w of them, in the order of the memory.  Sums, softmax
  * statistics and norms are fp32 whatever the dtype; an output is rounded once.  A tensor may be a channel range of a
  * wider one (its own c, the wider one's cpitch): channels beyond its own, rounded up to eight, stay as they are.
+ * Tensors, positions, masks and gains lie on the current device, and a call goes to one of its streams; an attention
+ * plan stays on the device it was made on (another one refuses its calls) and outlives the graphs that hold its calls.
+ * No call needs a workspace, allocates or waits for the device; any number of calls may be under way at once.
  * None of this has a counterpart in the reference. */
 
 #define DNB_ROPE_MAX_PAIRS 128
@@ -330,8 +333,9 @@ void dnb_attention_plan_destroy(dnb_attention_plan *plan);
  * states for all of q's where it is 1.  mask may be NULL.  A query that sees no key gets zeros.  y is no input's
  * memory.  Keys and values at and behind an image's length are not used, whatever they hold, and nor are those that a
  * mask with query_stride 0 hides; with a mask for each query, what only some of them may see has to be finite in v.
- * f32 operands are multiplied as sums of three bf16 numbers where a key head has more than 16 rows: an infinity, or a
- * number beyond bf16's largest (3.39e38), that a query sees makes NaN of the outputs that it reaches. */
+ * f32 operands are multiplied as sums of three bf16 numbers: magnitudes from 1.6e-33 to 3.38e38 keep their 24 bits, smaller
+ * ones lose some; an infinity, or a number beyond, that a query sees makes NaN of the outputs that it reaches.  At most
+ * 2^30 tokens an image. */
 int dnb_attention_forward(dnb_attention_plan *plan, const dnb_tensor *q, const dnb_tensor *k, const dnb_tensor *v,
                           const dnb_attention_mask *mask, const dnb_tensor *y, void *stream);
 
