@@ -332,7 +332,7 @@ void dnb_attention_plan_destroy(dnb_attention_plan *plan);
 /* y = softmax(scale q k^T) v.  q, y: [n][..][heads * head_dim]; k, v: [n or 1][..][kv_heads * head_dim], one image of
  * states for all of q's where it is 1.  mask may be NULL.  A query that sees no key gets zeros.  y is no input's
  * memory.  Keys and values at and behind an image's length are not used, whatever they hold, and nor are those that a
- * mask with query_stride 0 hides; with a mask for each query, what only some of them may see has to be finite in v.
+ * mask with query_stride 0 hides; with a mask for each query, every value in front of the length has to be finite.
  * f32 operands are multiplied as sums of three bf16 numbers: magnitudes from 1.6e-33 to 3.38e38 keep their 24 bits, smaller
  * ones lose some; an infinity, or a number beyond, that a query sees makes NaN of the outputs that it reaches.  At most
  * 2^30 tokens an image. */
