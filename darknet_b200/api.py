@@ -26,7 +26,7 @@ def _types():
     return _torch
 
 
-def _stream(stream=None):
+def _stream_number(stream=None) -> int:
     """The stream a call goes to, as a number: the caller's, or torch's current one.  torch.cuda.current_stream() makes a Python object of it, 3.2 us of the
     8.5 that the smallest call takes its host; torch's own handle of it is there in 0.2."""
     global _current
@@ -38,6 +38,10 @@ def _stream(stream=None):
         raw, device = getattr(torch._C, "_cuda_getCurrentRawStream", None), getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
         _current = (lambda: raw(device())) if raw else (lambda: torch.cuda.current_stream().cuda_stream)
     return _current()
+
+
+def _stream(stream=None) -> C.c_void_p:
+    return C.c_void_p(_stream_number(stream))
 
 
 def _function(name):
@@ -185,7 +189,7 @@ class RopePlan:
         """positions: int32 CUDA torch tensor [n * h * w, 3], or None for the tokens' places in the map."""
         if positions is not None:
             positions = _device_array(positions, (_types().int32,), (x.n * x.h * x.w, 3), "positions")
-        status = _function("dnb_rope_forward")(self.handle, C.byref(x), positions, C.byref(y), _stream(stream))
+        status = _function("dnb_rope_forward")(self.handle, C.byref(x), positions, C.byref(y), _stream_number(stream))
         if status:
             check(status)
 
@@ -223,7 +227,7 @@ class CrossAttentionPlan:
                     raise ValueError(f"mask: needs a CUDA tensor [{q.n}, {q.h * q.w}, {keys}] of bool or uint8 with contiguous keys")
                 masks.mask, masks.image_stride, masks.query_stride = mask.data_ptr(), mask.stride(0), mask.stride(1)
             masks = C.byref(masks)
-        status = _function("dnb_attention_forward")(self.handle, C.byref(q), C.byref(k), C.byref(v), masks, C.byref(y), _stream(stream))
+        status = _function("dnb_attention_forward")(self.handle, C.byref(q), C.byref(k), C.byref(v), masks, C.byref(y), _stream_number(stream))
         if status:
             check(status)
 
@@ -263,7 +267,7 @@ def rmsnorm(x: Tensor, y: Tensor | None = None, gain=None, eps=1e-6, residual: T
         pitch = e4m3.shape[-1]
         data = _device_array(e4m3, (_types().float8_e4m3fn, _types().uint8), (x.n, x.h, x.w, pitch), "e4m3")
         q = C.byref(E4M3(data, _device_array(scales, (_types().float32,), (x.n, x.h, x.w, -(-x.c // group) if group > 0 else 1), "scales"), pitch, group))
-    status = _function("dnb_rmsnorm_forward")(C.byref(x), _ref(residual), gain, eps, _ref(total), _ref(y), q, _stream(stream))
+    status = _function("dnb_rmsnorm_forward")(C.byref(x), _ref(residual), gain, eps, _ref(total), _ref(y), q, _stream_number(stream))
     if status:
         check(status)
 
