@@ -56,6 +56,27 @@ int check_tensor(const dnb_tensor *t, const char *what)
     return DNB_OK;
 }
 
+static size_t row_bytes(const dnb_tensor *t, int channels) { return (size_t)channels * (t->dtype == DNB_F32 ? 4 : 2); }
+static size_t span_bytes(const dnb_tensor *t)
+{
+    return ((size_t)t->n * t->h * t->w - 1) * row_bytes(t, t->cpitch) + row_bytes(t, (t->c + 7) / 8 * 8);
+}
+
+bool share_memory(const dnb_tensor *a, const dnb_tensor *b)
+{
+    if ((uintptr_t)a->data > (uintptr_t)b->data) { const dnb_tensor *t = a; a = b; b = t; }
+    const size_t apart = (uintptr_t)b->data - (uintptr_t)a->data;
+    if (apart >= span_bytes(a)) return false;
+    if (a->cpitch != b->cpitch) return true;
+    const size_t pitch = row_bytes(a, a->cpitch), at = apart % pitch;               // b's channels along a's rows
+    return at < row_bytes(a, (a->c + 7) / 8 * 8) || at + row_bytes(b, (b->c + 7) / 8 * 8) > pitch;
+}
+
+bool reaches_into(const dnb_tensor *t, const void *data, size_t bytes)
+{
+    return (uintptr_t)t->data < (uintptr_t)data + bytes && (uintptr_t)data < (uintptr_t)t->data + span_bytes(t);
+}
+
 }  // namespace dnb
 
 using namespace dnb;

@@ -54,6 +54,11 @@ int check_current_device(int device, const char *what);
 
 // Validation helpers (return DNB_OK or set the error).
 int check_tensor(const dnb_tensor *t, const char *what);
+// Whether two channels-last tensors of one dtype hold memory in common, their channels rounded up to eight.  Channel ranges of one wider tensor, of one pitch,
+// may lie between one another's rows.
+bool share_memory(const dnb_tensor *a, const dnb_tensor *b);
+// Whether a channels-last tensor reaches into `bytes` bytes at `data`.
+bool reaches_into(const dnb_tensor *t, const void *data, size_t bytes);
 inline size_t tensor_elems(const dnb_tensor *t)
 {
     return t->layout == DNB_NHWC ? (size_t)t->n * t->h * t->w * t->cpitch

@@ -192,7 +192,7 @@ extern "C" int dnb_attention_forward(dnb_attention_plan *p, const dnb_tensor *q,
     if (y->n != q->n || y->c != q->c || y->h != q->h || y->w != q->w) DNB_FAIL(DNB_EINVAL, "attention: queries and output differ in extents");
     if (k->n != q->n && k->n != 1) DNB_FAIL(DNB_EINVAL, "attention: keys of %d images for queries of %d (one for all, or one each)", k->n, q->n);
     for (const dnb_tensor *t : {q, k, v})
-        if (t->data == y->data) DNB_FAIL(DNB_EINVAL, "attention: the output is an input's memory");
+        if (share_memory(t, y)) DNB_FAIL(DNB_EINVAL, "attention: the output is an input's memory");
     if ((long long)q->h * q->w > 1LL << 30 || (long long)k->h * k->w > 1LL << 30) DNB_FAIL(DNB_EUNSUPPORTED, "attention: more than 2^30 tokens an image");
     AttnArgs a = {};
     a.q = q->data; a.k = k->data; a.v = v->data; a.y = y->data;

@@ -272,6 +272,10 @@ extern "C" int dnb_rmsnorm_forward(const dnb_tensor *x, const dnb_tensor *residu
     if (sum && y && sum->data == y->data) DNB_FAIL(DNB_EINVAL, "rmsnorm: sum and output are one tensor");
     for (const dnb_tensor *t : {sum, y})
         if (t && residual && t->data == residual->data && t->cpitch != residual->cpitch) DNB_FAIL(DNB_EINVAL, "rmsnorm: in place with another cpitch");
+    for (const dnb_tensor *t : {sum, y})
+        for (const dnb_tensor *in : {x, residual})
+            if (t && in && t->data != in->data && share_memory(t, in)) DNB_FAIL(DNB_EINVAL, "rmsnorm: an output is a part of an input's memory");
+    if (sum && y && share_memory(sum, y)) DNB_FAIL(DNB_EINVAL, "rmsnorm: sum and output share memory");
     if (gain && (uintptr_t)gain % 4) DNB_FAIL(DNB_EINVAL, "rmsnorm: gain must be 4-byte aligned");
     if (!(eps >= 0.f) || eps > 1e30f) DNB_FAIL(DNB_EINVAL, "rmsnorm: eps %g", (double)eps);
     NormArgs a = {};
@@ -280,8 +284,10 @@ extern "C" int dnb_rmsnorm_forward(const dnb_tensor *x, const dnb_tensor *residu
         if ((uintptr_t)q->data % 16 || (uintptr_t)q->scales % 4) DNB_FAIL(DNB_EINVAL, "rmsnorm: e4m3 data must be 16-byte aligned, its scales 4-byte aligned");
         if (q->pitch < x->c || q->pitch % 8) DNB_FAIL(DNB_EINVAL, "rmsnorm: e4m3 pitch %d for %d channels (need a multiple of 8 >= c)", q->pitch, x->c);
         if (q->group != 0 && q->group != 32 && q->group != 64 && q->group != 128) DNB_FAIL(DNB_EINVAL, "rmsnorm: groups of %d channels (0: one scale a token, 32, 64 or 128)", q->group);
+        const size_t tokens = (size_t)x->n * x->h * x->w, values = (tokens - 1) * q->pitch + round_up(x->c, 8), scales = tokens * (q->group ? (x->c + q->group - 1) / q->group : 1) * 4;
         for (const dnb_tensor *t : {x, residual, sum, y})
-            if (t && (t->data == q->data || t->data == (void *)q->scales)) DNB_FAIL(DNB_EINVAL, "rmsnorm: the e4m3 output is another tensor's memory");
+            if (t && (reaches_into(t, q->data, values) || reaches_into(t, q->scales, scales))) DNB_FAIL(DNB_EINVAL, "rmsnorm: the e4m3 output is another tensor's memory");
+        if ((uintptr_t)q->data < (uintptr_t)q->scales + scales && (uintptr_t)q->scales < (uintptr_t)q->data + values) DNB_FAIL(DNB_EINVAL, "rmsnorm: e4m3 values and scales share memory");
         a.q = (uint8_t *)q->data; a.scales = q->scales; a.qp = q->pitch; a.group = q->group;
         while (a.group >> a.group_log2 > 1) ++a.group_log2;
         a.groups = q->group ? (x->c + q->group - 1) / q->group : 1;

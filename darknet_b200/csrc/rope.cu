@@ -180,6 +180,7 @@ static int launch_rope(const dnb_rope_plan &p, const dnb_tensor *x, const int32_
     if (x->dtype != y->dtype || x->n != y->n || x->h != y->h || x->w != y->w || x->c != y->c) DNB_FAIL(DNB_EINVAL, "rope: input and output differ in dtype or extents");
     if ((long long)d.heads * d.head_dim > x->c) DNB_FAIL(DNB_EINVAL, "rope: %d heads of %d channels in a tensor of %d", d.heads, d.head_dim, x->c);
     if (x->data == y->data && x->cpitch != y->cpitch) DNB_FAIL(DNB_EINVAL, "rope: in place with another cpitch");
+    if (x->data != y->data && share_memory(x, y)) DNB_FAIL(DNB_EINVAL, "rope: the output is a part of the input's memory");
     if (positions && (uintptr_t)positions % 4) DNB_FAIL(DNB_EINVAL, "rope: positions must be 4-byte aligned");
     if (!positions && x->n % d.frames) DNB_FAIL(DNB_EINVAL, "rope: %d images are no whole number of clips of %d frames", x->n, d.frames);
     const long long tokens = (long long)x->n * x->h * x->w;
