@@ -395,7 +395,8 @@ attention_tc_kernel(const __grid_constant__ TcAttnArgs t)
                 mbar_wait_tight(smem_u32(&sh->o_full[s]), (j - 1) & 1, abort_flag, a.status, AT_OUTPUT, a.polls);
                 tc_fence_after();
             }
-            if (__any_sync(0xffffffffu, !((grown - top) * scale <= MOVE) && grown != -INFINITY)) {
+            // A row that no query fills has no say: its queries are what an earlier kernel left in shared memory, where the heads of a tile are no 128.
+            if (__any_sync(0xffffffffu, valid && !((grown - top) * scale <= MOVE) && grown != -INFINITY)) {
                 const float shrink = grown == top ? 1.f : ex2((top - grown) * scale);
                 if (j > 0) {
                     // each half its half of the channels (without a place of its own for P every product of the tile before has retired: the
