@@ -74,7 +74,7 @@ bool share_memory(const dnb_tensor *a, const dnb_tensor *b)
 
 bool reaches_into(const dnb_tensor *t, const void *data, size_t bytes)
 {
-    return (uintptr_t)t->data < (uintptr_t)data + bytes && (uintptr_t)data < (uintptr_t)t->data + span_bytes(t);
+    return ranges_meet(t->data, span_bytes(t), data, bytes);
 }
 
 }  // namespace dnb

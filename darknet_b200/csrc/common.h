@@ -57,7 +57,12 @@ int check_tensor(const dnb_tensor *t, const char *what);
 // Whether two channels-last tensors of one dtype hold memory in common, their channels rounded up to eight.  Channel ranges of one wider tensor, of one pitch,
 // may lie between one another's rows.
 bool share_memory(const dnb_tensor *a, const dnb_tensor *b);
-// Whether a channels-last tensor reaches into `bytes` bytes at `data`.
+// Whether `a_bytes` bytes at a and `b_bytes` at b have some in common.
+inline bool ranges_meet(const void *a, size_t a_bytes, const void *b, size_t b_bytes)
+{
+    return (uintptr_t)a < (uintptr_t)b + b_bytes && (uintptr_t)b < (uintptr_t)a + a_bytes;
+}
+// Whether a channels-last tensor, from its first byte to its last, reaches into `bytes` bytes at `data`.
 bool reaches_into(const dnb_tensor *t, const void *data, size_t bytes);
 inline size_t tensor_elems(const dnb_tensor *t)
 {

@@ -130,6 +130,22 @@ int cluster_room(const void *kernel, int slot, int threads, size_t smem, int roo
     return DNB_OK;
 }
 
+// Whether a tensor reaches into a mask's bytes: `queries` rows of `keys` bytes an image, at the mask's strides.
+static bool reaches_into_mask(const dnb_tensor *t, const dnb_attention_mask *m, int images, int queries, int keys)
+{
+    const __int128 image = images > 1 ? m->image_stride : 0, query = queries > 1 ? m->query_stride : 0, whole = (images - 1) * image + (queries - 1) * query + keys;
+    const uintptr_t at = (uintptr_t)m->mask;
+    if (!reaches_into(t, m->mask, whole > (__int128)(UINTPTR_MAX - at) ? (size_t)(UINTPTR_MAX - at) : (size_t)whole)) return false;
+    // between the first and the last byte: the first row of each image that ends behind the tensor's first byte, if there is one, decides
+    const __int128 begin = (__int128)(uintptr_t)t->data;
+    for (int i = 0; i < (image ? images : 1); ++i) {
+        const __int128 first = at + i * image, before = begin - first - keys;                // its own rows up to before / query end in front of the tensor
+        const __int128 j = before < 0 || !query ? 0 : before / query + 1, row = first + j * query;
+        if (j < queries && row <= (__int128)(UINTPTR_MAX - keys) && reaches_into(t, (const void *)(uintptr_t)row, (size_t)keys)) return true;
+    }
+    return false;
+}
+
 }  // namespace dnb
 
 using namespace dnb;
@@ -204,6 +220,8 @@ extern "C" int dnb_attention_forward(dnb_attention_plan *p, const dnb_tensor *q,
     if (mask) {
         if ((uintptr_t)mask->lengths % 4) DNB_FAIL(DNB_EINVAL, "attention: lengths must be 4-byte aligned");
         if (mask->mask && (mask->image_stride < 0 || mask->query_stride < 0)) DNB_FAIL(DNB_EINVAL, "attention: negative strides of the mask");
+        if (mask->lengths && reaches_into(y, mask->lengths, (size_t)q->n * 4)) DNB_FAIL(DNB_EINVAL, "attention: the output is the lengths' memory");
+        if (mask->mask && reaches_into_mask(y, mask, a.n, a.lq, a.lk)) DNB_FAIL(DNB_EINVAL, "attention: the output is the mask's memory");
         a.lengths = mask->lengths;
         a.mask = mask->mask; a.mask_image = mask->image_stride; a.mask_query = a.lq > 1 ? mask->query_stride : 0;   // one query: one mask for all of them
     }

@@ -277,6 +277,8 @@ extern "C" int dnb_rmsnorm_forward(const dnb_tensor *x, const dnb_tensor *residu
             if (t && in && t->data != in->data && share_memory(t, in)) DNB_FAIL(DNB_EINVAL, "rmsnorm: an output is a part of an input's memory");
     if (sum && y && share_memory(sum, y)) DNB_FAIL(DNB_EINVAL, "rmsnorm: sum and output share memory");
     if (gain && (uintptr_t)gain % 4) DNB_FAIL(DNB_EINVAL, "rmsnorm: gain must be 4-byte aligned");
+    for (const dnb_tensor *t : {sum, y})
+        if (t && gain && reaches_into(t, gain, (size_t)x->c * 4)) DNB_FAIL(DNB_EINVAL, "rmsnorm: an output is the gain's memory");
     if (!(eps >= 0.f) || eps > 1e30f) DNB_FAIL(DNB_EINVAL, "rmsnorm: eps %g", (double)eps);
     NormArgs a = {};
     if (q) {
@@ -287,7 +289,8 @@ extern "C" int dnb_rmsnorm_forward(const dnb_tensor *x, const dnb_tensor *residu
         const size_t tokens = (size_t)x->n * x->h * x->w, values = (tokens - 1) * q->pitch + round_up(x->c, 8), scales = tokens * (q->group ? (x->c + q->group - 1) / q->group : 1) * 4;
         for (const dnb_tensor *t : {x, residual, sum, y})
             if (t && (reaches_into(t, q->data, values) || reaches_into(t, q->scales, scales))) DNB_FAIL(DNB_EINVAL, "rmsnorm: the e4m3 output is another tensor's memory");
-        if ((uintptr_t)q->data < (uintptr_t)q->scales + scales && (uintptr_t)q->scales < (uintptr_t)q->data + values) DNB_FAIL(DNB_EINVAL, "rmsnorm: e4m3 values and scales share memory");
+        if (ranges_meet(q->data, values, q->scales, scales)) DNB_FAIL(DNB_EINVAL, "rmsnorm: e4m3 values and scales share memory");
+        if (gain && (ranges_meet(q->data, values, gain, (size_t)x->c * 4) || ranges_meet(q->scales, scales, gain, (size_t)x->c * 4))) DNB_FAIL(DNB_EINVAL, "rmsnorm: the e4m3 output is the gain's memory");
         a.q = (uint8_t *)q->data; a.scales = q->scales; a.qp = q->pitch; a.group = q->group;
         while (a.group >> a.group_log2 > 1) ++a.group_log2;
         a.groups = q->group ? (x->c + q->group - 1) / q->group : 1;

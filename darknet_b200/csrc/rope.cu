@@ -185,6 +185,7 @@ static int launch_rope(const dnb_rope_plan &p, const dnb_tensor *x, const int32_
     if (!positions && x->n % d.frames) DNB_FAIL(DNB_EINVAL, "rope: %d images are no whole number of clips of %d frames", x->n, d.frames);
     const long long tokens = (long long)x->n * x->h * x->w;
     if ((long long)x->n * x->h >= 1LL << 31 || tokens >= 1LL << 31) DNB_FAIL(DNB_EUNSUPPORTED, "rope: 2^31 tokens or more");
+    if (positions && reaches_into(y, positions, (size_t)tokens * 12)) DNB_FAIL(DNB_EINVAL, "rope: the output is the positions' memory");
     RopeArgs a;
     memcpy(a.turn, p.turn, sizeof(a.turn));
     a.x = x->data; a.y = y->data; a.positions = positions;

@@ -276,7 +276,8 @@ int dnb_softmax_forward(const dnb_tensor *x, const dnb_tensor *y, int groups, fl
  * Tensors, positions, masks and gains lie on the current device, and a call goes to one of its streams; an attention
  * plan stays on the device it was made on (another one refuses its calls) and outlives the graphs that hold its calls.
  * No call needs a workspace, allocates or waits for the device; any number of calls may be under way at once.
- * An output that shares memory with an input or another output is refused, but for those named below as in place.
+ * An output that shares memory with an input (positions, lengths, masks and gains among them) or another output is
+ * refused, but for those named below as in place.
  * None of this has a counterpart in the reference. */
 
 #define DNB_ROPE_MAX_PAIRS 128
