@@ -1,5 +1,7 @@
 // Internal argument blocks of the cross-attention kernels and the plan object.
 #pragma once
+#include <atomic>
+
 #include "common.h"
 
 struct dnb_attention_plan {
@@ -8,7 +10,7 @@ struct dnb_attention_plan {
     int *status;            // device word: 0, or the code of the bounded wait that ran out
     long long wait_limit;   // SM clock cycles
     int debug;
-    const char *kernel;     // of the last forward, for logs and tests
+    std::atomic<const char *> kernel;   // of the last forward of any thread, for logs and tests
 };
 
 namespace dnb {

@@ -4,6 +4,8 @@
 
 #include <string.h>
 
+#include <atomic>
+
 namespace dnb {
 
 static thread_local char g_error[512] = "";
@@ -19,15 +21,15 @@ const char *get_error() { return g_error; }
 
 int sm_count()
 {
-    static int cached[64];
+    static std::atomic<int> cached[64];
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-    if (!cached[dev]) {
-        int v = 0;
+    int v = cached[dev].load(std::memory_order_relaxed);
+    if (!v) {
         if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v <= 0) v = 148;
-        cached[dev] = v;
+        cached[dev].store(v, std::memory_order_relaxed);
     }
-    return cached[dev];
+    return v;
 }
 
 int check_current_device(int device, const char *what)

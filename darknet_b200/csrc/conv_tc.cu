@@ -1055,9 +1055,8 @@ static int max_pair_clusters(K kernel, size_t smem, int threads)
 // DNB_PDL=0 launches every kernel plainly (no overlap of a kernel's set-up with the tail of the kernel before it).
 bool pdl_enabled()
 {
-    static int v = -1;
-    if (v < 0) { const char *e = getenv("DNB_PDL"); v = e ? (atoi(e) != 0) : 1; }
-    return v != 0;
+    static const bool v = [] { const char *e = getenv("DNB_PDL"); return e ? atoi(e) != 0 : true; }();
+    return v;
 }
 
 // One launch.  Single CTAs: one CTA per SM slot (or per tile, if fewer).  Pair mode: clusters of two CTAs, as many as are
@@ -1215,13 +1214,14 @@ static CUresult with_context(F encode)
 int encode_tensor_map(CUtensorMap *map, int elem_kind, int rank, void *base, const uint64_t *dims,
                       const uint64_t *strides_bytes, const uint32_t *box, int swizzle_bytes)
 {
-    static EncodeTiledFn fn = nullptr;
+    static std::atomic<EncodeTiledFn> known;
+    EncodeTiledFn fn = known.load(std::memory_order_relaxed);
     if (!fn) {
         void *p = nullptr;
         cudaDriverEntryPointQueryResult q;
         DNB_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q));
         if (!p || q != cudaDriverEntryPointSuccess) DNB_FAIL(DNB_ECUDA, "cuTensorMapEncodeTiled is not available from this driver");
-        fn = (EncodeTiledFn)p;
+        known.store(fn = (EncodeTiledFn)p, std::memory_order_relaxed);
     }
     cuuint64_t d[5], st[4];
     cuuint32_t bx[5], es[5];

@@ -179,7 +179,7 @@ extern "C" int dnb_attention_plan_create(const dnb_attention_desc *desc, dnb_att
     if (p->d.scale == 0.f) p->d.scale = 1.f / sqrtf((float)d.head_dim);
     p->device = device;
     p->status = status;
-    p->kernel = "none";
+    p->kernel.store("none", std::memory_order_relaxed);
     *plan = p;
     return DNB_OK;
 }
@@ -232,18 +232,18 @@ extern "C" int dnb_attention_forward(dnb_attention_plan *p, const dnb_tensor *q,
     if (p->device < 0) DNB_FAIL(DNB_ECUDA, "attention: the plan was made without a CUDA device");
     DNB_TRY(check_current_device(p->device, "attention"));
     if (attention_rows_covers(a)) {
-        p->kernel = q->dtype == DNB_F32 ? "rows_f32" : "rows_bf16";
+        p->kernel.store(q->dtype == DNB_F32 ? "rows_f32" : "rows_bf16", std::memory_order_relaxed);
         return launch_attention_rows(a, q->dtype, (cudaStream_t)stream);
     }
     if (attention_f32_tc_covers(a, q->dtype)) {
-        p->kernel = "tc_f32";
+        p->kernel.store("tc_f32", std::memory_order_relaxed);
         return launch_attention_f32_tc(a, (cudaStream_t)stream);
     }
     if (attention_tc_covers(a, q->dtype)) {
-        p->kernel = "tc_bf16";
+        p->kernel.store("tc_bf16", std::memory_order_relaxed);
         return launch_attention_tc(a, (cudaStream_t)stream);
     }
-    p->kernel = "simple";
+    p->kernel.store("simple", std::memory_order_relaxed);
     return launch_attention_simple(a, q->dtype, (cudaStream_t)stream);
 }
 
@@ -268,4 +268,4 @@ extern "C" int dnb_attention_plan_set_diagnostics(dnb_attention_plan *p, long lo
     return DNB_OK;
 }
 
-extern "C" const char *dnb_attention_plan_kernel(const dnb_attention_plan *p) { return p ? p->kernel : "none"; }
+extern "C" const char *dnb_attention_plan_kernel(const dnb_attention_plan *p) { return p ? p->kernel.load(std::memory_order_relaxed) : "none"; }
