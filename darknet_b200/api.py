@@ -13,6 +13,7 @@ from . import (ACTIVATIONS, BF16, E4M3, F32, MODE_TF32, NCHW, NHWC, AttentionDes
 
 
 _current = None
+_device = None
 _functions = {}
 _torch = None
 
@@ -33,11 +34,20 @@ def _stream_number(stream=None) -> int:
     if stream is not None:
         return int(stream)
     if _current is None:
-        import torch
-        torch.cuda.current_device()                   # torch's first use of the device
-        raw, device = getattr(torch._C, "_cuda_getCurrentRawStream", None), getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
-        _current = (lambda: raw(device())) if raw else (lambda: torch.cuda.current_stream().cuda_stream)
+        _device_number()
+        raw = getattr(_types()._C, "_cuda_getCurrentRawStream", None)
+        _current = (lambda: raw(_device())) if raw else (lambda: _types().cuda.current_stream().cuda_stream)
     return _current()
+
+
+def _device_number() -> int:
+    """The current device."""
+    global _device
+    if _device is None:
+        torch = _types()
+        torch.cuda.current_device()                   # torch's first use of the device
+        _device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+    return _device()
 
 
 def _stream(stream=None) -> C.c_void_p:
@@ -166,9 +176,16 @@ def softmax(x: Tensor, y: Tensor, groups: int = 1, temperature: float = 1.0, str
 
 
 def _device_array(t, dtypes, shape, what):
-    """The address of a contiguous CUDA tensor of one of `dtypes` and of `shape`."""
+    """The address of a contiguous CUDA tensor of one of `dtypes` and of `shape`, on the current device."""
     if not t.is_cuda or t.dtype not in dtypes or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{what}: needs a contiguous CUDA tensor {list(shape)} of {' or '.join(str(d) for d in dtypes)}")
+    return _address(t, what)
+
+
+def _address(t, what):
+    """The address of a CUDA tensor; a kernel on the current device could not read another one's."""
+    if t.get_device() != _device_number():
+        raise ValueError(f"{what}: lies on CUDA device {t.get_device()}, device {_device_number()} is current")
     return t.data_ptr()
 
 
@@ -225,7 +242,7 @@ class CrossAttentionPlan:
                 keys = k.h * k.w
                 if not mask.is_cuda or mask.dtype not in (_types().bool, _types().uint8) or mask.shape != (q.n, q.h * q.w, keys) or (keys > 1 and mask.stride(2) != 1):
                     raise ValueError(f"mask: needs a CUDA tensor [{q.n}, {q.h * q.w}, {keys}] of bool or uint8 with contiguous keys")
-                masks.mask, masks.image_stride, masks.query_stride = mask.data_ptr(), mask.stride(0), mask.stride(1)
+                masks.mask, masks.image_stride, masks.query_stride = _address(mask, "mask"), mask.stride(0), mask.stride(1)
             masks = C.byref(masks)
         status = _function("dnb_attention_forward")(self.handle, C.byref(q), C.byref(k), C.byref(v), masks, C.byref(y), _stream_number(stream))
         if status:
