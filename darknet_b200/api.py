@@ -278,6 +278,8 @@ def rmsnorm(x: Tensor, y: Tensor | None = None, gain=None, eps=1e-6, residual: T
     gain: float32 CUDA torch tensor [c].  e4m3: float8_e4m3fn (or uint8) CUDA torch tensor [n, h, w, pitch] with scales, a float32 one
     [n, h, w, groups]; group: channels that share a scale (32, 64, 128), or 0 for all."""
     q = None
+    if (e4m3 is None) != (scales is None):
+        raise ValueError("e4m3 and scales: one comes with the other")
     if gain is not None:
         gain = _device_array(gain, (_types().float32,), (x.c,), "gain")
     if e4m3 is not None:

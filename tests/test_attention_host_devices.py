@@ -61,3 +61,12 @@ def test_arrays_on_another_device(what, reached):
     assert not reached
     call(1)
     assert len(reached) == 1
+
+
+def test_values_in_8_bits_come_with_their_scales(reached):
+    x = tensor(2, 3, 3, 60)
+    with pytest.raises(ValueError, match="scales"):
+        dn.rmsnorm(x, x, e4m3=OnDevice(1, torch.uint8, 2, 3, 3, 64), stream=0)
+    with pytest.raises(ValueError, match="scales"):                         # they would stay as they are
+        dn.rmsnorm(x, x, scales=OnDevice(1, torch.float32, 2, 3, 3, 1), stream=0)
+    assert not reached
