@@ -159,7 +159,7 @@ extern "C" int dnb_attention_plan_create(const dnb_attention_desc *desc, dnb_att
     if (d.head_dim < 8 || d.head_dim % 8) DNB_FAIL(DNB_EINVAL, "attention: heads of %d channels (need a multiple of 8)", d.head_dim);
     if (d.head_dim > 128) DNB_FAIL(DNB_EUNSUPPORTED, "attention: heads of %d channels (at most 128)", d.head_dim);
     if ((long long)d.heads * d.head_dim >= 1LL << 24) DNB_FAIL(DNB_EUNSUPPORTED, "attention: %d heads of %d channels", d.heads, d.head_dim);
-    if (!isfinite(d.scale)) DNB_FAIL(DNB_EINVAL, "attention: scale is not finite");
+    if (!isfinite(d.scale * LOG2E)) DNB_FAIL(DNB_EINVAL, "attention: scale %g (times log2 e it has to be finite)", (double)d.scale);   // exponentials are taken to base 2
     // Without a device the plan still checks the arguments of its calls, and then refuses them.
     int device = -1, *status = nullptr;
     if (cudaGetDevice(&device) != cudaSuccess || cudaMalloc(&status, sizeof(int)) != cudaSuccess) {

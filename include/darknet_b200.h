@@ -311,7 +311,8 @@ int dnb_rope_forward(const dnb_rope_plan *plan, const dnb_tensor *x, const int32
                      void *stream);
 
 /* Attention of q's tokens to k's and v's: heads query heads, kv_heads of keys and values, query head i reads head
- * i / (heads / kv_heads).  scale 0 stands for 1 / sqrt(head_dim).  head_dim: a multiple of 8, at most 128. */
+ * i / (heads / kv_heads).  scale 0 stands for 1 / sqrt(head_dim); scale * log2(e) has to be finite.  head_dim: a
+ * multiple of 8, at most 128. */
 typedef struct dnb_attention_desc {
     int heads, kv_heads, head_dim;
     float scale;
