@@ -211,7 +211,7 @@ attention_f32_tc_kernel(const __grid_constant__ F32TcArgs t)
                 }
                 fence_async_smem();
                 __syncwarp();
-                if (*abort_flag) break;
+                if (gave_up(abort_flag)) break;
                 if (lane == 0 && !(a.debug & 32 && is_v)) mbar_arrive(smem_u32(&full[stage]));
                 if (++stage == C::STAGES) { stage = 0; phase ^= 1; }
             }

@@ -194,7 +194,7 @@ attention_tc_kernel(const __grid_constant__ TcAttnArgs t)
             uint32_t phase = 0;
             for (int i = 0; i < 2 * tiles; ++i) {
                 const uint32_t full = smem_u32(&sh->full[stage]);
-                if (!mbar_wait_known(smem_u32(&sh->empty[stage]), phase ^ 1, abort_flag, a.status, AT_SLOT, a.polls)) break;
+                if (!mbar_wait_known(smem_u32(&sh->empty[stage]), phase ^ 1, abort_flag, a.status, AT_SLOT, a.polls) || gave_up(abort_flag)) break;
                 if (elect_one() && !(a.debug & 32 && i == 1)) {
                     mbar_expect_tx(full, C::TILE_BYTES);
                     for (int b = 0; b < C::BOXES; ++b)

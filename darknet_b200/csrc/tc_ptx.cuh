@@ -135,6 +135,9 @@ __device__ __forceinline__ bool mbar_wait_known(uint32_t bar, uint32_t parity, v
     mbar_wait_tight(bar, parity, abort_flag, status, code, polls);
     return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) && !__any_sync(0xffffffffu, *abort_flag != 0);
 }
+// Whether a wait of the block has run out, the same for the whole warp.  A warp that fills slots asks before each: those that empty them go on over whatever is
+// there, and a slot would be filled again before its last load has landed.
+__device__ __forceinline__ bool gave_up(volatile int *abort_flag) { return __any_sync(0xffffffffu, *abort_flag != 0); }
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1, int c2, int c3)
 {
