@@ -271,7 +271,8 @@ int dnb_softmax_forward(const dnb_tensor *x, const dnb_tensor *y, int groups, fl
 /* What a language or query head on a detector's feature map needs beside the 1x1 convolutions that project its
  * tokens: rotary positions, attention to the map's pixels, and the norm between the blocks.  Channels-last tensors of
  * one dtype (f32 or bf16); a token is a pixel, n * h * w of them, in the order of the memory.  Sums, softmax
- * statistics and norms are fp32 whatever the dtype; an output is rounded once.  A tensor may be a channel range of a
+ * statistics and norms are fp32 whatever the dtype; an output is rounded once.  Attention of bf16 tensors rounds its
+ * softmax weights to bf16 as well, where they meet the values (their sum is that of the unrounded ones).  A tensor may be a channel range of a
  * wider one (its own c, the wider one's cpitch): channels beyond its own, rounded up to eight, stay as they are.
  * Tensors, positions, masks and gains lie on the current device, and a call goes to one of its streams; an attention
  * plan stays on the device it was made on (another one refuses its calls) and outlives the graphs that hold its calls.
@@ -306,7 +307,8 @@ int dnb_rope_plan_create(const dnb_rope_desc *desc, dnb_rope_plan **plan);
 void dnb_rope_plan_destroy(dnb_rope_plan *plan);
 
 /* y = x with its heads turned; y may be x (then what passes is not touched).  positions: device int32
- * [n * h * w][3], or NULL.  Angles are exact modulo a turn for every int32 position. */
+ * [n * h * w][3], or NULL.  Angles are taken modulo a turn, off by 2^-30 of one at most for every int32 position where
+ * |scale * f| is at most 1 (beyond that by as much more as it is larger). */
 int dnb_rope_forward(const dnb_rope_plan *plan, const dnb_tensor *x, const int32_t *positions, const dnb_tensor *y,
                      void *stream);
 
@@ -333,16 +335,19 @@ int dnb_attention_plan_create(const dnb_attention_desc *desc, dnb_attention_plan
 void dnb_attention_plan_destroy(dnb_attention_plan *plan);
 
 /* y = softmax(scale q k^T) v.  q, y: [n][..][heads * head_dim]; k, v: [n or 1][..][kv_heads * head_dim], one image of
- * states for all of q's where it is 1.  mask may be NULL.  A query that sees no key gets zeros.  y is no input's
- * memory.  Keys and values at and behind an image's length are not used, whatever they hold, and nor are those that a
+ * states for all of q's where it is 1.  mask may be NULL.  A query that sees no key, or none whose score is above
+ * -infinity, gets zeros.  y is no input's memory.  Keys and values at and behind an image's length are not used, whatever they hold, and nor are those that a
  * mask with query_stride 0 hides; with a mask for each query, every value in front of the length has to be finite.
  * f32 operands are multiplied as sums of three bf16 numbers: magnitudes from 1.6e-33 to 3.38e38 keep their 24 bits, smaller
- * ones lose some; an infinity, or a number beyond, that a query sees makes NaN of the outputs that it reaches.  At most
- * 2^30 tokens an image. */
+ * ones lose some; an infinity, or a number beyond, that a query sees makes NaN of the outputs that it reaches (where
+ * more than 128 query heads share a key head, sums are plain fp32 ones, and such numbers stay what those make of
+ * them).  At most 2^30 tokens an image. */
 int dnb_attention_forward(dnb_attention_plan *plan, const dnb_tensor *q, const dnb_tensor *k, const dnb_tensor *v,
                           const dnb_attention_mask *mask, const dnb_tensor *y, void *stream);
 
-/* dnb_conv_plan_check_status and dnb_conv_plan_set_diagnostics of an attention plan; the kernel of its last call. */
+/* dnb_conv_plan_check_status and dnb_conv_plan_set_diagnostics of an attention plan; the kernel of its last call, of
+ * whatever host thread.  The status is that of calls whose stream has been waited for; diagnostics are set while no
+ * other thread calls. */
 int dnb_attention_plan_check_status(dnb_attention_plan *plan);
 int dnb_attention_plan_set_diagnostics(dnb_attention_plan *plan, long long wait_limit_cycles, int debug_bits);
 const char *dnb_attention_plan_kernel(const dnb_attention_plan *plan);
@@ -358,7 +363,8 @@ typedef struct dnb_e4m3 {
 /* s = x + residual;  y = s * rsqrt(mean over c of s^2 + eps) * gain;  q = y / scale with scale = max(max |y| of the
  * group / 448, 2^-126).  residual, gain (device fp32 [c], or 1), sum (s as stored), y and q may each be NULL, but not
  * all outputs, nor residual with a sum asked for.  The norm takes s before its rounding.  sum and y may each be x's or
- * residual's own memory.  c: at most 32768 (bf16) or 16384 (f32). */
+ * residual's own memory.  c: at most 32768 (bf16) or 16384 (f32); eps from 0 to 1e30.  Squares are fp32: a token whose
+ * sum of them overflows (magnitudes of 2^64 and more) gets zeros, NaN where it is infinite itself. */
 int dnb_rmsnorm_forward(const dnb_tensor *x, const dnb_tensor *residual, const float *gain, float eps,
                         const dnb_tensor *sum, const dnb_tensor *y, const dnb_e4m3 *q, void *stream);
 

@@ -57,3 +57,16 @@ def test_tokens_behind_the_first(dtype, vecs, tokens, less, group):
     values = q[0, 0, :, :c].contiguous().view(torch.float8_e4m3fn).double() * got
     within(values, want, want.abs() * (2.0 ** -4 + 2 * e) + got * 2.0 ** -10, "8 bits")
     assert bool((q[..., c:] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_squares_that_overflow(dtype):
+    """Squares are fp32: 2^63 over 3 channels has a norm, 2^64 has zeros, with an infinity beside them NaN there."""
+    x = torch.zeros((1, 1, 3, 8), dtype=TORCH[dtype], device="cuda")
+    x[0, 0, 0, :3], x[0, 0, 1, :3] = 2.0 ** 63, 2.0 ** 64
+    x[0, 0, 2, :3] = torch.tensor([2.0 ** 64, float("inf"), -1.0])
+    y, q, scales = torch.full_like(x, 7.0), torch.full((1, 1, 3, 8), 0x11, dtype=torch.uint8, device="cuda"), torch.zeros((1, 1, 3, 1), device="cuda")
+    dn.rmsnorm(dn.as_tensor(x, dn.NHWC, 3), dn.as_tensor(y, dn.NHWC, 3), None, 1e-6, e4m3=q, scales=scales)
+    assert bool(((y[0, 0, 0, :3].double() - 1).abs() <= HALF[dtype] + norm_error(3)).all())
+    assert bool((y[0, 0, 1] == 0).all()) and bool((q[0, 0, 1] == 0).all()) and scales[0, 0, 1].item() == 2.0 ** -126
+    assert torch.isnan(y[0, 0, 2, :3]).tolist() == [False, True, False] and bool((y[0, 0, 2, [0, 2]] == 0).all()) and bool((y[..., 3:] == 0).all())
