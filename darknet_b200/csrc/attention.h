@@ -31,7 +31,7 @@ struct AttnArgs {
     int debug;
 };
 
-// How many CTAs share the keys of one job (1, 2, 4 or 8: a cluster).  A wave of CTAs takes its tiles of keys, `start` tiles' time to begin and end, and
+// How many CTAs share the keys of one job (1, 2, 4 or 8: a cluster), as if every image had all its keys.  A wave of CTAs takes its tiles of keys, `start` tiles' time to begin and end, and
 // `join` tiles' for each CTA that joins; room[i]: the CTAs of clusters of 2^i that run at once.
 int split_keys(long long jobs, int key_tiles, const int room[4], double start, double join);
 // room of a kernel of one CTA an SM, asked once a device and slot (0 .. 7)

@@ -17,7 +17,9 @@ namespace dnb {
 constexpr float LOG2E = 1.4426950408889634f;
 
 // One warp a query and head: 32 keys at a time, a key a lane for the scores, a few channels a lane for the sum of the values, the largest score and
-// the sum of the weights as they go.  Right for every case.
+// the sum of the weights as they go.  Right for every case; what is left to it are more than 128 heads a key head, more than a tile of the others holds.
+// A lane's loads of its key, one channel after another, bound it: 8 tokens, 160 heads of 64 over one key head and 1444 keys, 829 us in bf16 and 946 in f32,
+// where 128 heads take the tensor cores 10 and 19.
 template <typename T>
 __global__ void __launch_bounds__(128)
 attention_simple_kernel(const __grid_constant__ AttnArgs a)

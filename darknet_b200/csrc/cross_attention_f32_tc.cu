@@ -10,7 +10,7 @@
 // the weights (half a row a thread) and add the tiles up, four split the keys into parts, four the values, one issues the products.  S and P have two places
 // each, so that a tile's scores are made while the tile before is weighed.  A tile's chain of hand-overs bounds it, 1.9 us of 64 keys and heads of 64 (the
 // products alone would take 0.8), 4.6 of heads of 128, whose keys and values have one place each beside three parts of queries.
-// Measured: 8 x 100 queries over 1444 keys, 8 heads of 32, 25 us; 4 x 2000 over 5776, 8 heads of 64, 692 us (137 TFLOP/s of f32 products; 32 on the CUDA cores).
+// Measured: 8 x 100 queries over 1444 keys, 8 heads of 32, 25 us (28 with a mask for each query); 4 x 2000 over 5776, 8 heads of 64, 652 us (145 TFLOP/s of f32 products; 32 on the CUDA cores).
 // Few rows: the keys are split over the CTAs of a cluster, which join their sums through distributed shared memory.
 #include <atomic>
 
@@ -438,7 +438,8 @@ int launch_attention_f32_tc(const AttnArgs &a, cudaStream_t stream)
     const int key_tiles = (a.lk + KEYS - 1) / KEYS;
     const size_t bytes = tmem_smem(a.mask ? (a.d > 64 ? F32TcCfg<128, true>::BYTES : F32TcCfg<64, true>::BYTES) : a.d > 64 ? F32TcCfg<128, false>::BYTES : F32TcCfg<64, false>::BYTES, 512);
     // Heads of 64, us over 1 / 2 / 4 / 8 CTAs a job: 8 jobs of 6 tiles 17.6 / 14.3 / 12.6 / 15.1, 32 jobs of 23 49.0 / 31.5 / 21.6 / 51.6, 200 jobs of 91
-    // 360 / 295 / 380.  A tile's time is 1.9 us (4.6 of heads of 128).
+    // 360 / 295 / 380.  A tile's time is 1.9 us (4.6 of heads of 128); one pair of constants serves both.  The images' own lengths are on the device and do not
+    // count: 256 jobs of up to 91 tiles 283 / 265 / 316, as chosen 283.
     int room[4];
     DNB_TRY(cluster_room((const void *)kern, 4 + which, THREADS, bytes, room));
     t.splits = split_keys(jobs, key_tiles, room, 3.0, 0.5);

@@ -382,6 +382,11 @@ template <typename T, int DP> RowsVariant rows_variant() { return {attention_row
 
 }  // namespace
 
+// Up to the 16 rows of its one product.  us of this kernel / of the one for 128 rows at 16 rows, which costs that one what one row or 128 do (8 key heads):
+//   4 images of 5776 keys, heads of 64  bf16 13.9 / 20.3  f32 28.5 / 51.1     heads of 128  bf16 23.4 / 27.5  f32 49.6 / 110
+//   8 of 1444                           bf16 10.3 / 13.2  f32 17.0 / 29.9                   bf16 15.1 / 17.1  f32 29.4 / 62.5
+//   1 of 361                            bf16  6.6 / 6.7   f32  6.1 / 10.7                   bf16 10.1 / 8.3   f32  9.4 / 18.4   (at 8 rows bf16 7.7 / 8.3)
+// A second product of 16 rows, for up to 32, is not there: from 17 rows on the right-hand figures hold.
 bool attention_rows_covers(const AttnArgs &a)
 {
     return a.d <= 128 && (long long)a.lq * a.group <= 16 && (long long)a.n * a.kv_heads < 1LL << 28;

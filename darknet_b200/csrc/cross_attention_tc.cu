@@ -6,7 +6,8 @@
 //   P = exp2(S * scale * log2 e - m)   eight warps a tile, half a row a thread, out of TMEM and back into it as bf16
 //   O += P V    tcgen05.mma, P from TMEM, V from shared memory as it lies (channels innermost: a transposed operand), O in TMEM (fp32)
 // While one tile's warps take exponentials, the tensor cores multiply the other tile's: the two are never both idle.
-// Measured: 8 x 5776 queries over 5776 keys, 8 heads of 128 916 us (1190 TFLOP/s, tensor pipe and exponentials 58 % each), of 64 710 us (770 TFLOP/s): there
+// Measured: 8 x 5776 queries over 5776 keys, 8 heads of 128 916 us on a cool GPU (1190 TFLOP/s, tensor pipe and exponentials 58 % each) and 1055 to 1073 us
+// (1020 TFLOP/s) in a run of seconds, under the power cap; of 64 710 us (770 TFLOP/s): there
 // the softmax's chain bounds it (exponentials for nothing would save 4 %; a share of them as polynomials on the FMA pipe costs 4 to 10 %).
 //
 // The running maximum m moves only when a row's largest score has outgrown it by more than 2^8 (every weight is then at most 256 times what
@@ -564,7 +565,8 @@ int launch_attention_tc(const AttnArgs &a, cudaStream_t stream)
     DNB_TRY(prepare(kern, which));
     const size_t bytes = tmem_smem(a.mask ? (a.d > 64 ? Cfg<128, true>::BYTES : Cfg<64, true>::BYTES) : a.d > 64 ? Cfg<128, false>::BYTES : Cfg<64, false>::BYTES, 512);
     // Heads of 64, us over 1 / 2 / 4 / 8 CTAs a job: 8 jobs of 3 tiles 9.5 / 11.4 / 13.5, of 12 22.8 / 17.0 / 15.1 / 19.3, of 46 69.7 / 41.2 / 27.8 / 25.4;
-    // 152 jobs of 46 144 / 128 / 145, 384 jobs of 46 216 / 249.  A tile's time is 1.4 us (1.8 of heads of 128).
+    // 152 jobs of 46 144 / 128 / 145, 384 jobs of 46 216 / 249.  A tile's time is 1.4 us (1.8 of heads of 128); one pair of constants serves both.  The images' own
+    // lengths are on the device and do not count: 128 jobs of up to 46 tiles 73.4 / 72.9 / 99.2, as chosen 73.4.
     int room[4];
     DNB_TRY(cluster_room((const void *)kern, which, THREADS, bytes, room));
     t.splits = a.mask ? split_keys(jobs, key_tiles, room, 2.5, 0.6) : split_keys(jobs, key_tiles, room, 4.0, 1.0);   // a masked tile takes 1.7 times as long
